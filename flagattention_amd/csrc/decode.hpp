@@ -73,6 +73,36 @@ FA_DEVICE int thread_for_output() {
   return (int)t;
 }
 
+// The 4 wavefronts' results for the workgroup's 16 rows, left in area[w][row] as D values, the maximum (in units of 1 / c2
+// in the base-2 exponent) and the sum, become one result per row.
+template <int D>
+FA_DEVICE void merge_wavefronts(const float* area, int n_rows, float c2, DecodeOut<D>& out) {
+  constexpr int ROWS = 16, RS = D + 2;
+  hw::block_sync();
+  const int out_tid = thread_for_output();
+#pragma unroll
+  for (int e = 0; e < DecodeOut<D>::kPerThread; ++e) {
+    if (e * kThreads / D < n_rows) {   // uniform: a GQA group of 4 reads a quarter of the area
+      const int idx = out_tid + e * kThreads;
+      const int row = (idx / D) % ROWS, d = idx % D;  // idx >= 16 * D occurs only when 16 * D < 256; callers skip it
+      float mw[4], mm = neg_inf();
+#pragma unroll
+      for (int w = 0; w < 4; ++w) { mw[w] = area[(w * ROWS + row) * RS + D]; mm = fmaxf(mm, mw[w]); }
+      const float m_use = (mm == neg_inf()) ? 0.f : mm;
+      float acc = 0.f, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = hw::exp2_fast((mw[w] - m_use) * c2);  // -inf -> 0
+        acc += f * area[(w * ROWS + row) * RS + d];
+        sum += f * area[(w * ROWS + row) * RS + D + 1];
+      }
+      out.o[e] = acc;
+      out.row_max[e] = mm;
+      out.row_sum[e] = sum;
+    }
+  }
+}
+
 // A load instruction of a step covers RPI consecutive keys (64 lanes of 16 bytes).  Src must provide:
 //   struct Ids;                                             lookup state for one step
 //   void lookup(Ids&, int n0, int n_last, int lane) const;  start resolving the rows of the step at key n0 (at most n_last)
@@ -296,29 +326,7 @@ FA_DEVICE void decode_block(const Src& src, const T* q_row /* query row of lane 
       for (int r = 0; r < 4; ++r) mine[16 * db + 4 * g + r] = oacc[db][r];
     if (g == 0) { mine[D] = m_i; mine[D + 1] = l_i; }
   }
-  hw::block_sync();
-  const int out_tid = thread_for_output();
-#pragma unroll
-  for (int e = 0; e < DecodeOut<D>::kPerThread; ++e) {
-    if (e * kThreads / D < n_rows) {   // uniform: a GQA group of 4 reads a quarter of the area
-      const int idx = out_tid + e * kThreads;
-      const int row = (idx / D) % C::ROWS, d = idx % D;  // idx >= 16 * D occurs only when 16 * D < 256; callers skip it
-      float mw[4], mm = neg_inf();
-#pragma unroll
-      for (int w = 0; w < 4; ++w) { mw[w] = area[(w * C::ROWS + row) * RS + D]; mm = fmaxf(mm, mw[w]); }
-      const float m_use = (mm == neg_inf()) ? 0.f : mm;
-      float acc = 0.f, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = hw::exp2_fast((mw[w] - m_use) * c2);  // -inf -> 0
-        acc += f * area[(w * C::ROWS + row) * RS + d];
-        sum += f * area[(w * C::ROWS + row) * RS + D + 1];
-      }
-      out.o[e] = acc;
-      out.row_max[e] = mm;
-      out.row_sum[e] = sum;
-    }
-  }
+  merge_wavefronts<D>(area, n_rows, c2, out);
 }
 
 }  // namespace fa
