@@ -313,6 +313,69 @@ def paged_reduce(lib, out, tmp_out, max_logits, exp_sums, context_lens, Hkv, par
                            int(partition_size), int(num_parts), stream_of(out)), "paged_reduce")
 
 
+def used_stride(t, dim):
+    """The stride of a dimension of extent 1 is never used; torch leaves arbitrary values there."""
+    return t.stride(dim) if t.shape[dim] > 1 else 0
+
+
+def paged_attn_e4m3(lib, out, query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables, scale,
+                    workspace, num_workgroups):
+    """workspace None and num_workgroups 0: one workgroup per sequence, kv head and 16 query heads."""
+    num_seqs, Hq, D = query.shape
+    num_blocks, Hkv, block_size, _ = key_cache.shape
+    check(lib.paged_attn_e4m3(dtype_code(query), ptr(out), out.stride(0), out.stride(1),
+                              ptr(query), used_stride(query, 0), used_stride(query, 1), ptr(key_cache), ptr(value_cache),
+                              used_stride(key_cache, 0), used_stride(key_cache, 1), used_stride(key_cache, 2),
+                              ptr(key_scales), ptr(value_scales), key_scales.stride(0), key_scales.stride(1),
+                              ptr(context_lens), ptr(block_tables), int(block_tables.dtype == torch.int64),
+                              block_tables.stride(0), block_tables.shape[1], num_blocks, float(scale), num_seqs, Hq, Hkv, D,
+                              block_size, ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size(),
+                              int(num_workgroups), stream_of(query)), "paged_attn_e4m3")
+
+
+def paged_append(lib, key, value, key_cache, value_cache, key_scales, value_scales, context_lens, starts, block_tables, cos,
+                 sin, interleaved):
+    """starts None: one row per sequence; scales None: a cache of the rows' type; cos, sin None: no rotation."""
+    rows, Hkv, D = key.shape
+    num_blocks, _, block_size, _ = key_cache.shape
+    scale_strides = (0, 0) if key_scales is None else key_scales.stride()
+    table = (0, 0, 0) if cos is None else (cos.stride(0), cos.shape[0], 2 * cos.shape[1])
+    check(lib.paged_append(dtype_code(key), ptr(key), used_stride(key, 0), used_stride(key, 1), ptr(value), used_stride(value, 0),
+                           used_stride(value, 1), ptr(key_cache), ptr(value_cache), used_stride(key_cache, 0), used_stride(key_cache, 1),
+                           used_stride(key_cache, 2), ptr(key_scales), ptr(value_scales), *scale_strides, ptr(context_lens),
+                           ptr(starts), ptr(block_tables), int(block_tables.dtype == torch.int64), block_tables.stride(0),
+                           block_tables.shape[1], num_blocks, ptr(cos), ptr(sin), *table, int(interleaved), rows,
+                           block_tables.shape[0], Hkv, D, block_size, stream_of(key)), "paged_append")
+
+
+def _rotary_tail(cos, sin, positions, interleaved, eps, shape, kv_heads):
+    B, H, T, D = shape
+    pos = (0, 0, 0) if positions is None else \
+        (int(positions.dtype == torch.int64), used_stride(positions, 0), used_stride(positions, 1))
+    return (ptr(cos), ptr(sin), cos.stride(0), cos.shape[0], 2 * cos.shape[1], int(interleaved), ptr(positions), *pos,
+            float(eps), B, H, kv_heads, T, D)
+
+
+def fa_norm_rotary(lib, q, k, q_out, k_out, q_weight, k_weight, cos, sin, positions, interleaved, eps):
+    """positions (B, T) or None."""
+    check(lib.fa_norm_rotary(dtype_code(q), view4(q), view4(k), view4(q_out), view4(k_out), ptr(q_weight), ptr(k_weight),
+                             int(q_weight is not None and q_weight.dtype == torch.float32),
+                             *_rotary_tail(cos, sin, positions, interleaved, eps, q.shape, k.shape[1]), stream_of(q)),
+          "fa_norm_rotary")
+
+
+def fa_norm_rotary_bwd(lib, q, k, dq_out, dk_out, dq, dk, q_weight, k_weight, dq_weight, dk_weight, workspace, cos, sin,
+                       positions, interleaved, eps):
+    """Without weights q, k, the weights' gradients and the workspace are None."""
+    inputs = (None, None) if q_weight is None else (view4(q), view4(k))
+    check(lib.fa_norm_rotary_bwd(dtype_code(dq), *inputs, view4(dq_out), view4(dk_out), view4(dq), view4(dk), ptr(q_weight),
+                                 ptr(k_weight), ptr(dq_weight), ptr(dk_weight),
+                                 int(q_weight is not None and q_weight.dtype == torch.float32),
+                                 *_rotary_tail(cos, sin, positions, interleaved, eps, dq.shape, dk.shape[1]), ptr(workspace),
+                                 0 if workspace is None else workspace.numel() * workspace.element_size(), stream_of(dq)),
+          "fa_norm_rotary_bwd")
+
+
 def fa_probe_mfma(lib, sink, iters, random_operands=True, dtype=torch.bfloat16):
     """Enqueues the matrix-pipe rate probe on ``sink``'s device; returns the FLOP the launch executes."""
     code = F16 if dtype == torch.float16 else BF16

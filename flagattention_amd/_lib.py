@@ -54,6 +54,15 @@ SIGNATURES = {
     "paged_attn_balanced_workspace": [_i, _i],
     "paged_attn_balanced": [_i, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i, _i64,
                             _f, _i, _i, _i, _i, _i, _p, _i64, _i, _p],
+    "paged_attn_e4m3": [_i, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i, _i64,
+                        _i, _i, _f, _i, _i, _i, _i, _i, _p, _i64, _i, _p],
+    "paged_append": [_i, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p, _i, _i64,
+                     _i, _i, _p, _p, _i64, _i64, _i, _i, _i64, _i, _i, _i, _i, _p],
+    "fa_norm_rotary": [_i, _v, _v, _v, _v, _p, _p, _i, _p, _p, _i64, _i64, _i, _i, _p, _i, _i64, _i64, _f, _i, _i, _i, _i,
+                       _i, _p],
+    "fa_norm_rotary_workspace": [_i],
+    "fa_norm_rotary_bwd": [_i, _v, _v, _v, _v, _v, _v, _p, _p, _p, _p, _i, _p, _p, _i64, _i64, _i, _i, _p, _i, _i64, _i64,
+                           _f, _i, _i, _i, _i, _i, _p, _i64, _p],
     "fa_probe_mfma": [_i, _i, _i, _p, _i64, _p],
     "paged_attn_balanced_static_prepare": [],
     "paged_attn_balanced_static": [_i, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i, _i64,
@@ -104,7 +113,7 @@ class PythonForm:
     def _not_taken(*args):
         return NotImplemented
 
-    flash = piecewise = paged = _not_taken
+    flash = piecewise = paged = paged_fp8 = paged_append = norm_rotary = _not_taken
 
 
 _native = None

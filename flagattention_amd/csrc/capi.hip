@@ -522,6 +522,137 @@ int paged_attn_balanced_static(int dtype, void* out, int64_t o_stride_s, int64_t
                              num_kv_heads, head_size, block_size, ws, need, num_workgroups, stream);
 }
 
+static bool paged_head_size_ok(int D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256 || D == 512; }
+
+int paged_attn_e4m3(int dtype, void* out, int64_t o_stride_s, int64_t o_stride_h, const void* query,
+                    int64_t q_stride_s, int64_t q_stride_h, const void* key_cache, const void* value_cache,
+                    int64_t kv_stride_blk, int64_t kv_stride_h, int64_t kv_stride_tok, const float* key_scales,
+                    const float* value_scales, int64_t scale_stride_blk, int64_t scale_stride_h,
+                    const int32_t* context_lens, const void* block_tables, int bt_is_int64, int64_t bt_stride,
+                    int bt_cols, int num_blocks, float attn_scale, int num_seqs, int num_q_heads, int num_kv_heads,
+                    int head_size, int block_size, void* workspace, int64_t workspace_bytes, int num_workgroups,
+                    void* stream) {
+  fa::PagedParams p = {};
+  const int rc = fill_paged(p, dtype, out, o_stride_s, o_stride_h, context_lens, num_seqs, num_q_heads,
+                            num_kv_heads, head_size, 0, 1, nullptr, nullptr, nullptr);
+  if (rc) return rc;
+  if (!query || !key_cache || !value_cache || !block_tables || !key_scales || !value_scales) return FA_ERR_BAD_ARGUMENT;
+  if ((((uintptr_t)query) | ((uintptr_t)key_cache) | ((uintptr_t)value_cache) | ((uintptr_t)workspace)) & 15) return FA_ERR_BAD_ARGUMENT;
+  if ((((uintptr_t)key_scales) | ((uintptr_t)value_scales)) & 3) return FA_ERR_BAD_ARGUMENT;
+  if ((q_stride_s | q_stride_h) % 8 || (kv_stride_blk | kv_stride_h | kv_stride_tok) % 16) return FA_ERR_BAD_ARGUMENT;
+  if (!paged_head_size_ok(head_size)) return FA_ERR_UNSUPPORTED;
+  if (num_workgroups < 0) return FA_ERR_BAD_ARGUMENT;
+  if (num_workgroups > 0 && (!workspace || workspace_bytes < fa::paged_balanced_workspace_bytes(num_workgroups, head_size)))
+    return FA_ERR_BAD_ARGUMENT;
+  p.q = query; p.q_ss = q_stride_s; p.q_sh = q_stride_h;
+  p.kc = key_cache; p.vc = value_cache;
+  p.kv_sblk = kv_stride_blk; p.kv_sh = kv_stride_h; p.kv_stok = kv_stride_tok;
+  p.k_scales = key_scales; p.v_scales = value_scales;
+  p.scale_sblk = scale_stride_blk; p.scale_sh = scale_stride_h;
+  p.block_tables = block_tables; p.bt64 = bt_is_int64; p.bt_stride = bt_stride;
+  p.bt_cols = bt_cols; p.num_blocks = num_blocks;
+  p.scale = attn_scale; p.block_size = block_size;
+  p.ws = (float*)workspace; p.num_wgs = num_workgroups;
+  return fa::run_paged_e4m3(p, (hipStream_t)stream);
+}
+
+// tables of a rotation, where there is one
+static bool tables_ok(const float* cos, const float* sin, int64_t stride, int64_t rows) {
+  return cos && sin && !((((uintptr_t)cos) | ((uintptr_t)sin)) & 15) && stride % 4 == 0 && rows > 0;
+}
+
+int paged_append(int dtype, const void* key, int64_t k_stride_r, int64_t k_stride_h, const void* value,
+                 int64_t v_stride_r, int64_t v_stride_h, void* key_cache, void* value_cache, int64_t kv_stride_blk,
+                 int64_t kv_stride_h, int64_t kv_stride_tok, float* key_scales, float* value_scales,
+                 int64_t scale_stride_blk, int64_t scale_stride_h, const int32_t* context_lens, const int32_t* starts,
+                 const void* block_tables, int bt_is_int64, int64_t bt_stride, int bt_cols, int num_blocks,
+                 const float* cos, const float* sin, int64_t table_stride, int64_t table_rows, int rotary_size,
+                 int interleaved, int64_t rows, int num_seqs, int num_kv_heads, int head_size, int block_size,
+                 void* stream) {
+  if (!key || !value || !key_cache || !value_cache || !context_lens || !block_tables) return FA_ERR_BAD_ARGUMENT;
+  if (!key_scales != !value_scales) return FA_ERR_BAD_ARGUMENT;
+  if ((((uintptr_t)key) | ((uintptr_t)value) | ((uintptr_t)key_cache) | ((uintptr_t)value_cache)) & 15) return FA_ERR_BAD_ARGUMENT;
+  if ((((uintptr_t)key_scales) | ((uintptr_t)value_scales)) & 3) return FA_ERR_BAD_ARGUMENT;
+  if ((k_stride_r | k_stride_h | v_stride_r | v_stride_h) % 8) return FA_ERR_BAD_ARGUMENT;
+  if ((kv_stride_blk | kv_stride_h | kv_stride_tok) % (key_scales ? 16 : 8)) return FA_ERR_BAD_ARGUMENT;
+  if (rotary_size != 0 && !tables_ok(cos, sin, table_stride, table_rows)) return FA_ERR_BAD_ARGUMENT;
+  if (!paged_head_size_ok(head_size)) return FA_ERR_UNSUPPORTED;
+  fa::AppendParams p = {};
+  p.side[0] = {key, k_stride_r, k_stride_h, key_cache, key_scales};
+  p.side[1] = {value, v_stride_r, v_stride_h, value_cache, value_scales};
+  p.c_blk = kv_stride_blk; p.c_head = kv_stride_h; p.c_tok = kv_stride_tok;
+  p.s_blk = scale_stride_blk; p.s_head = scale_stride_h;
+  p.lens = context_lens; p.starts = starts;
+  p.block_tables = block_tables; p.bt64 = bt_is_int64; p.bt_stride = bt_stride; p.bt_cols = bt_cols;
+  p.cos = cos; p.sin = sin; p.table_stride = table_stride; p.table_rows = table_rows;
+  p.rows = rows; p.num_blocks = num_blocks; p.num_seqs = num_seqs; p.Hkv = num_kv_heads;
+  p.D = head_size; p.block_size = block_size;
+  p.rotary = rotary_size; p.interleaved = interleaved; p.dtype = dtype;
+  return fa::run_append(p, (hipStream_t)stream);
+}
+
+// what both directions of fa_norm_rotary take
+static int fill_rotary(fa::RotaryParams& p, int dtype, const void* q_weight, const void* k_weight, int weights_f32,
+                       const float* cos, const float* sin, int64_t table_stride, int64_t table_rows, int rotary_size,
+                       int interleaved, const void* positions, int positions_int64, int64_t pos_stride_b,
+                       int64_t pos_stride_t, float eps, int B, int H, int Hk, int T, int D) {
+  if (!q_weight != !k_weight) return FA_ERR_BAD_ARGUMENT;
+  if ((((uintptr_t)q_weight) | ((uintptr_t)k_weight)) & (weights_f32 ? 3 : 1)) return FA_ERR_BAD_ARGUMENT;
+  if (((uintptr_t)positions) & (positions_int64 ? 7 : 3)) return FA_ERR_BAD_ARGUMENT;
+  if (!tables_ok(cos, sin, table_stride, table_rows)) return FA_ERR_BAD_ARGUMENT;
+  if (!paged_head_size_ok(D)) return FA_ERR_UNSUPPORTED;
+  p.side[0].w = q_weight; p.side[0].heads = H;
+  p.side[1].w = k_weight; p.side[1].heads = Hk;
+  p.cos = cos; p.sin = sin; p.table_stride = table_stride; p.table_rows = table_rows;
+  p.positions = positions; p.pos64 = positions_int64; p.pos_sb = pos_stride_b; p.pos_st = pos_stride_t;
+  p.eps = eps; p.B = B; p.T = T; p.D = D;
+  p.rotary = rotary_size; p.interleaved = interleaved; p.w_f32 = weights_f32; p.dtype = dtype;
+  return 0;
+}
+
+int fa_norm_rotary(int dtype, const fa_view4* q, const fa_view4* k, const fa_view4* q_out, const fa_view4* k_out,
+                   const void* q_weight, const void* k_weight, int weights_f32, const float* cos, const float* sin,
+                   int64_t table_stride, int64_t table_rows, int rotary_size, int interleaved, const void* positions,
+                   int positions_int64, int64_t pos_stride_b, int64_t pos_stride_t, float eps, int B, int H, int Hk,
+                   int T, int D, void* stream) {
+  if (!view_ok(q) || !view_ok(k) || !view_ok(q_out) || !view_ok(k_out)) return FA_ERR_BAD_ARGUMENT;
+  fa::RotaryParams p = {};
+  const int rc = fill_rotary(p, dtype, q_weight, k_weight, weights_f32, cos, sin, table_stride, table_rows, rotary_size,
+                             interleaved, positions, positions_int64, pos_stride_b, pos_stride_t, eps, B, H, Hk, T, D);
+  if (rc) return rc;
+  p.side[0].x = to_view(q); p.side[0].y = to_view(q_out);
+  p.side[1].x = to_view(k); p.side[1].y = to_view(k_out);
+  return fa::run_rotary(p, (hipStream_t)stream);
+}
+
+int fa_norm_rotary_workspace(int D) {
+  if (!paged_head_size_ok(D)) return FA_ERR_UNSUPPORTED;
+  return (int)fa::rotary_workspace_bytes(D);
+}
+
+int fa_norm_rotary_bwd(int dtype, const fa_view4* q, const fa_view4* k, const fa_view4* dq_out, const fa_view4* dk_out,
+                       const fa_view4* dq, const fa_view4* dk, const void* q_weight, const void* k_weight,
+                       void* dq_weight, void* dk_weight, int weights_f32, const float* cos, const float* sin,
+                       int64_t table_stride, int64_t table_rows, int rotary_size, int interleaved,
+                       const void* positions, int positions_int64, int64_t pos_stride_b, int64_t pos_stride_t,
+                       float eps, int B, int H, int Hk, int T, int D, void* workspace, int64_t workspace_bytes,
+                       void* stream) {
+  if (!view_ok(dq_out) || !view_ok(dk_out) || !view_ok(dq) || !view_ok(dk)) return FA_ERR_BAD_ARGUMENT;
+  fa::RotaryParams p = {};
+  const int rc = fill_rotary(p, dtype, q_weight, k_weight, weights_f32, cos, sin, table_stride, table_rows, rotary_size,
+                             interleaved, positions, positions_int64, pos_stride_b, pos_stride_t, eps, B, H, Hk, T, D);
+  if (rc) return rc;
+  if (q_weight) {
+    if (!view_ok(q) || !view_ok(k) || !dq_weight || !dk_weight || !workspace) return FA_ERR_BAD_ARGUMENT;
+    if ((((uintptr_t)dq_weight) | ((uintptr_t)dk_weight)) & (weights_f32 ? 3 : 1)) return FA_ERR_BAD_ARGUMENT;
+    if (((uintptr_t)workspace) & 15 || workspace_bytes < fa::rotary_workspace_bytes(D)) return FA_ERR_BAD_ARGUMENT;
+  }
+  p.side[0].x = to_view(q); p.side[0].dy = to_view(dq_out); p.side[0].y = to_view(dq); p.side[0].dw = dq_weight;
+  p.side[1].x = to_view(k); p.side[1].dy = to_view(dk_out); p.side[1].y = to_view(dk); p.side[1].dw = dk_weight;
+  p.partial = (float*)workspace;
+  return fa::run_rotary_bwd(p, (hipStream_t)stream);
+}
+
 int fa_probe_mfma(int dtype, int random_operands, int iters, float* sink, int64_t sink_floats, void* stream) {
   const int cus = fa::num_cus_of_current_device();
   if (cus <= 0) return FA_ERR_UNSUPPORTED;

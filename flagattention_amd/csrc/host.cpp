@@ -1,12 +1,12 @@
 // Host path of the operators for GPU tensors: argument checks, launch decisions, allocations and launches of one
-// call in one native function, with native autograd nodes for the two operators that have gradients.
+// call in one native function, with native autograd nodes for the operators that have gradients.
 //
 // Why it is native: the kernels of a short call take 10-40 us, and the same work done in Python through ctypes took
 // longer than they do -- 38 us for a decode step, 20 us for a paged one, 195 us for a forward and backward over
 // 512 tokens (of 42 us of kernels).
 //
 // The Python modules hold the reference form of the launch decisions made here (`flash.py`, `split_kv.py`, `paged.py`,
-// `piecewise.py`).  It runs whenever a tile-config hook has been replaced, for tensors that are not on a GPU, where
+// `piecewise.py`, `paged_fp8.py`, `append.py`, `rotary.py`).  It runs whenever a tile-config hook has been replaced, for tensors that are not on a GPU, where
 // this extension is not built, and for every call this file does not take (it then answers NotImplemented, before any
 // effect); arguments that are in error are among those, so that their messages have one source.  `decisions()` and the
 // functions after it expose the numbers chosen here to the tests that compare them with the Python functions.  One
@@ -738,6 +738,271 @@ PyObject* paged(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------ around the paged cache ----
+bool head_size_ok(int64_t D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256 || D == 512; }
+
+// two caches of one layout that the kernels take as they are (append.check_cache_layout)
+bool caches_ok(const Tensor& kc, const Tensor& vc, const Tensor& first) {
+  if (!is_operand(kc, kc) || !is_operand(vc, kc) || kc.device() != first.device() || vc.sizes() != kc.sizes() || vc.strides() != kc.strides() ||
+      kc.stride(3) != 1 || (((uintptr_t)kc.const_data_ptr() | (uintptr_t)vc.const_data_ptr()) & 15))
+    return false;
+  const int64_t align = 16 / (int64_t)kc.element_size();
+  for (int i = 0; i < 3; ++i)
+    if (kc.size(i) > 1 && kc.stride(i) % align) return false;
+  return fits_int({kc.size(0), kc.size(1), kc.size(2)});
+}
+// the stride of a dimension of extent 1 is never used; torch leaves arbitrary values there
+int64_t used_stride(const Tensor& t, int dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
+// scales of an e4m3 cache (append.check_cache)
+bool scales_ok(const Tensor& kc, const Tensor& ks, const Tensor& vs) {
+  for (const Tensor* t : {&ks, &vs})
+    if (!t->is_cuda() || t->layout() != at::kStrided || t->device() != kc.device() || t->scalar_type() != at::kFloat || t->dim() != 2 ||
+        t->size(0) != kc.size(0) || t->size(1) != kc.size(1) || t->strides() != ks.strides())
+      return false;
+  return kc.scalar_type() == at::kFloat8_e4m3fn;
+}
+bool int32_ready(const Tensor& t, const Tensor& first, int64_t n) {
+  return t.scalar_type() == at::kInt && t.device() == first.device() && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+}
+bool table_ready(const Tensor& bt, const Tensor& first, int64_t seqs) {
+  return bt.device() == first.device() && bt.layout() == at::kStrided && bt.dim() == 2 && bt.size(0) == seqs && bt.stride(1) == 1 &&
+         (bt.scalar_type() == at::kInt || bt.scalar_type() == at::kLong) && fits_int({bt.size(1)});
+}
+// cos and sin as append.tables_ready leaves them
+bool tables_ready(const Tensor& cos, const Tensor& sin, const Tensor& first, int64_t D) {
+  for (const Tensor* t : {&cos, &sin})
+    if (!t->is_cuda() || t->layout() != at::kStrided || t->device() != first.device() || t->scalar_type() != at::kFloat || t->dim() != 2 ||
+        t->sizes() != cos.sizes() || t->strides() != cos.strides() || t->stride(1) != 1 || t->stride(0) % 4 || ((uintptr_t)t->const_data_ptr() & 15))
+      return false;
+  const int64_t size = 2 * cos.size(1);
+  return size > 0 && size <= D && size % 16 == 0 && cos.size(0) > 0;
+}
+bool rows3_ready(const Tensor& t) { return t.dim() == 3 && t.layout() == at::kStrided && is_kernel_ready(t); }
+// an argument that may be None; false: it is neither that nor a plain tensor
+bool optional_tensor(PyObject* a, const Tensor*& t) {
+  t = nullptr;
+  if (a == Py_None) return true;
+  if (!THPVariable_CheckExact(a)) return false;
+  t = &THPVariable_Unpack(a);
+  return plain_call({t});
+}
+
+// paged_fp8(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables, attn_scale, max_context_len)
+PyObject* paged_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 9, "paged_fp8: nine arguments");
+  if (!plain_tensors(a, 7)) return not_taken();
+  const Tensor &q = THPVariable_Unpack(a[0]), &kc = THPVariable_Unpack(a[1]), &vc = THPVariable_Unpack(a[2]), &ks = THPVariable_Unpack(a[3]),
+               &vs = THPVariable_Unpack(a[4]), &lens = THPVariable_Unpack(a[5]), &bt = THPVariable_Unpack(a[6]);
+  if (!plain_call({&q, &kc, &vc, &ks, &vs, &lens, &bt})) return not_taken();
+  if (!q.is_cuda() || !rows3_ready(q) || !type_ok(q) || !caches_ok(kc, vc, q) || !scales_ok(kc, ks, vs)) return not_taken();
+  const int64_t seqs = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = kc.size(1), block = kc.size(2);
+  if (!fits_int({seqs, Hq}) || kc.size(3) != D || Hq % Hkv || !head_size_ok(D) || !int32_ready(lens, q, seqs) || !table_ready(bt, q, seqs))
+    return not_taken();
+  const double scale = PyFloat_AsDouble(a[7]);
+  const long long longest = PyLong_Check(a[8]) ? PyLong_AsLongLong(a[8]) : -1;
+  if (PyErr_Occurred()) { PyErr_Clear(); return not_taken(); }
+  if (longest < 0) return not_taken();
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(q.device());
+    out = empty_result(q);
+    const int wgs = balanced_workgroups(seqs, Hkv, Hq / Hkv, D, longest, fa_num_cus());
+    const int64_t bytes = wgs > 0 ? paged_attn_balanced_workspace(wgs, (int)D) : 0;
+    Tensor ws = wgs > 0 ? empty({bytes / 4}, at::kFloat, q) : Tensor();
+    check(paged_attn_e4m3(dtype_code(q), out.mutable_data_ptr(), out.stride(0), out.stride(1), q.const_data_ptr(), used_stride(q, 0),
+                          used_stride(q, 1), kc.const_data_ptr(), vc.const_data_ptr(), used_stride(kc, 0), used_stride(kc, 1), used_stride(kc, 2),
+                          f32(ks), f32(vs), ks.stride(0), ks.stride(1), (const int32_t*)lens.const_data_ptr(), bt.const_data_ptr(),
+                          bt.scalar_type() == at::kLong, bt.stride(0), (int)bt.size(1), (int)kc.size(0), (float)scale, (int)seqs, (int)Hq,
+                          (int)Hkv, (int)D, (int)block, wgs > 0 ? ws.mutable_data_ptr() : nullptr, bytes, wgs, stream_of(q)),
+          "paged_attn_e4m3");
+  }
+  return THPVariable_Wrap(out);
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_append(key, value, key_cache, value_cache, context_lens, block_tables, query_starts, key_scales, value_scales, cos, sin,
+//              interleaved)
+PyObject* paged_append_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 12, "paged_append: twelve arguments");
+  if (!plain_tensors(a, 6)) return not_taken();
+  const Tensor &k = THPVariable_Unpack(a[0]), &v = THPVariable_Unpack(a[1]), &kc = THPVariable_Unpack(a[2]), &vc = THPVariable_Unpack(a[3]),
+               &lens = THPVariable_Unpack(a[4]), &bt = THPVariable_Unpack(a[5]);
+  const Tensor *starts, *ks, *vs, *cos, *sin;
+  if (!optional_tensor(a[6], starts) || !optional_tensor(a[7], ks) || !optional_tensor(a[8], vs) || !optional_tensor(a[9], cos) ||
+      !optional_tensor(a[10], sin) || !plain_call({&k, &v, &kc, &vc, &lens, &bt}))
+    return not_taken();
+  const int interleaved = PyObject_IsTrue(a[11]);
+  if (interleaved < 0) throw python_error();
+  if (!k.is_cuda() || v.device() != k.device() || !rows3_ready(k) || !rows3_ready(v) || !type_ok(k) || v.scalar_type() != k.scalar_type() ||
+      v.sizes() != k.sizes() || !caches_ok(kc, vc, k))
+    return not_taken();
+  const int64_t rows = k.size(0), Hkv = k.size(1), D = k.size(2), seqs = bt.dim() == 2 ? bt.size(0) : 0;
+  if (!fits_int({rows, Hkv, seqs}) || kc.size(1) != Hkv || kc.size(3) != D || !head_size_ok(D) || !table_ready(bt, k, seqs) ||
+      !int32_ready(lens, k, seqs) || (starts ? !int32_ready(*starts, k, seqs + 1) : rows != seqs))
+    return not_taken();
+  if ((ks == nullptr) != (vs == nullptr) || (ks ? !scales_ok(kc, *ks, *vs) : kc.scalar_type() != k.scalar_type())) return not_taken();
+  if ((cos == nullptr) != (sin == nullptr) || (cos && !tables_ready(*cos, *sin, k, D))) return not_taken();
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(k.device());
+    check(paged_append(dtype_code(k), k.const_data_ptr(), used_stride(k, 0), used_stride(k, 1), v.const_data_ptr(), used_stride(v, 0),
+                       used_stride(v, 1), kc.mutable_data_ptr(), vc.mutable_data_ptr(), used_stride(kc, 0), used_stride(kc, 1), used_stride(kc, 2),
+                       ks ? f32(*ks) : nullptr, vs ? f32(*vs) : nullptr, ks ? ks->stride(0) : 0, ks ? ks->stride(1) : 0,
+                       (const int32_t*)lens.const_data_ptr(), starts ? (const int32_t*)starts->const_data_ptr() : nullptr, bt.const_data_ptr(),
+                       bt.scalar_type() == at::kLong, bt.stride(0), (int)bt.size(1), (int)kc.size(0), cos ? f32(*cos) : nullptr,
+                       cos ? f32(*sin) : nullptr, cos ? cos->stride(0) : 0, cos ? cos->size(0) : 0, cos ? (int)(2 * cos->size(1)) : 0,
+                       interleaved, rows, (int)seqs, (int)Hkv, (int)D, (int)kc.size(2), stream_of(k)), "paged_append");
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// ------------------------------------------------------------------------------------------ norm and rotation ----
+struct RotaryCall {
+  bool interleaved;
+  double eps;
+};
+// what both directions pass on besides the tensors of (B, heads, T, D)
+struct RotaryTables {
+  Tensor wq, wk, cos, sin, positions;   // undefined: none
+  int f32_weights() const { return wq.defined() && wq.scalar_type() == at::kFloat; }
+  const void* at(const Tensor& t) const { return t.defined() ? t.const_data_ptr() : nullptr; }
+  int64_t pos_stride(int dim) const { return positions.defined() ? used_stride(positions, dim) : 0; }
+  int pos64() const { return positions.defined() && positions.scalar_type() == at::kLong; }
+};
+
+struct RotaryNode : torch::autograd::Function<RotaryNode> {
+  static variable_list run(const Tensor& q, const Tensor& k, const RotaryTables& t, const RotaryCall& c) {
+    Tensor qo = empty_result(q), ko = empty_result(k);
+    const fa_view4 a = view4(q), b = view4(k), x = view4(qo), y = view4(ko);
+    check(fa_norm_rotary(dtype_code(q), &a, &b, &x, &y, t.at(t.wq), t.at(t.wk), t.f32_weights(), f32(t.cos), f32(t.sin), t.cos.stride(0),
+                         t.cos.size(0), (int)(2 * t.cos.size(1)), c.interleaved, t.at(t.positions), t.pos64(), t.pos_stride(0), t.pos_stride(1),
+                         (float)c.eps, (int)q.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), (int)q.size(3), stream_of(q)),
+          "fa_norm_rotary");
+    return {qo, ko};
+  }
+  // (the weights again as arguments, for their gradients; an autograd function takes no undefined tensor but in an optional)
+  static variable_list forward(AutogradContext* ctx, const Tensor& q0, const Tensor& k0, const std::optional<Tensor>& wq,
+                               const std::optional<Tensor>& wk, const RotaryTables& t, const RotaryCall& c) {
+    const Tensor q = kernel_ready(q0), k = kernel_ready(k0);
+    variable_list out = run(q, k, t, c);
+    const bool normed = t.wq.defined();   // a rotation alone is undone without its input
+    ctx->save_for_backward({normed ? q : Tensor(), normed ? k : Tensor(), t.wq, t.wk, t.cos, t.sin, t.positions});
+    ctx->saved_data["q"] = q.sizes();
+    ctx->saved_data["k"] = k.sizes();
+    hold(ctx, c);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const RotaryCall& c = held<RotaryCall>(ctx);
+    const RotaryTables t{s[2], s[3], s[4], s[5], s[6]};
+    const auto qs = ctx->saved_data["q"].toIntVector(), kshape = ctx->saved_data["k"].toIntVector();
+    const Tensor& some = grads[0].defined() ? grads[0] : grads[1];
+    if (!some.defined()) return variable_list(6);
+    const c10::DeviceGuard guard(some.device());
+    // the gradient of an output that nothing flows into is zero
+    const Tensor gq = grads[0].defined() ? kernel_ready(grads[0]) : at::zeros(qs, some.options()),
+                 gk = grads[1].defined() ? kernel_ready(grads[1]) : at::zeros(kshape, some.options());
+    Tensor dq = empty(qs, gq.scalar_type(), gq), dk = empty(kshape, gq.scalar_type(), gq), dwq, dwk, ws;
+    const fa_view4 vgq = view4(gq), vgk = view4(gk), vdq = view4(dq), vdk = view4(dk);
+    fa_view4 vq = {}, vk = {};
+    const int D = (int)qs[3];
+    int64_t bytes = 0;
+    if (t.wq.defined()) {
+      vq = view4(s[0]);
+      vk = view4(s[1]);
+      dwq = empty({D}, t.wq.scalar_type(), gq);
+      dwk = empty({D}, t.wk.scalar_type(), gq);
+      bytes = fa_norm_rotary_workspace(D);
+      ws = empty({bytes / 4}, at::kFloat, gq);
+    }
+    check(fa_norm_rotary_bwd(dtype_code(gq), &vq, &vk, &vgq, &vgk, &vdq, &vdk, t.at(t.wq), t.at(t.wk), dwq.defined() ? dwq.mutable_data_ptr() : nullptr,
+                             dwk.defined() ? dwk.mutable_data_ptr() : nullptr, t.f32_weights(), f32(t.cos), f32(t.sin), t.cos.stride(0), t.cos.size(0),
+                             (int)(2 * t.cos.size(1)), c.interleaved, t.at(t.positions), t.pos64(), t.pos_stride(0), t.pos_stride(1),
+                             (float)c.eps, (int)qs[0], (int)qs[1], (int)kshape[1], (int)qs[2], D, ws.defined() ? ws.mutable_data_ptr() : nullptr,
+                             bytes, stream_of(gq)), "fa_norm_rotary_bwd");
+    return {dq, dk, dwq, dwk, Tensor(), Tensor()};
+  }
+};
+
+// A leaf's gradient is handed over on the stream that its autograd node was made on.  A node that an eager graph keeps alive
+// is tied to that graph's stream: a captured backward that reached it would draw the stream into the capture, which ends the
+// process when the capture ends.  So a call that a capture is to record is refused for such leaves.
+void check_capture(std::initializer_list<const Tensor*> ts) {
+  const auto stream = c10::hip::getCurrentHIPStream();
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  for (const Tensor* t : ts) {
+    if (!t || !t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto on = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!on || on->id() == stream.id(),
+                "norm_rotary: an input that requires a gradient is held by an autograd graph of another stream, and the backward "
+                "of this call cannot be captured while that graph lives; release it, or capture without gradients");
+  }
+}
+
+// norm_rotary(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved)
+PyObject* norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK(n == 9, "norm_rotary: nine arguments");
+  if (!plain_tensors(a, 4)) return not_taken();
+  const Tensor &q0 = THPVariable_Unpack(a[0]), &k0 = THPVariable_Unpack(a[1]), &cos = THPVariable_Unpack(a[2]), &sin = THPVariable_Unpack(a[3]);
+  const Tensor *pos, *wq, *wk;
+  if (!optional_tensor(a[4], pos) || !optional_tensor(a[5], wq) || !optional_tensor(a[6], wk) || !plain_call({&q0, &k0, &cos, &sin})) return not_taken();
+  const int interleaved = PyObject_IsTrue(a[8]);
+  if (interleaved < 0) throw python_error();
+  RotaryCall c = {interleaved != 0, PyFloat_AsDouble(a[7])};
+  if (PyErr_Occurred()) { PyErr_Clear(); return not_taken(); }
+  if (!q0.is_cuda() || q0.layout() != at::kStrided || k0.layout() != at::kStrided || (q0.dim() != 3 && q0.dim() != 4) || k0.dim() != q0.dim() ||
+      k0.device() != q0.device() || k0.scalar_type() != q0.scalar_type() || !type_ok(q0))
+    return not_taken();
+  const bool single = q0.dim() == 3;
+  if (single && (!pos || pos->dim() != 1)) return not_taken();
+  const int64_t B = q0.size(0), H = q0.size(1), T = single ? 1 : q0.size(2), D = q0.size(-1), Hk = k0.size(1);
+  if (!fits_int({B, H, T, Hk, B * T}) || k0.size(0) != B || k0.size(-1) != D || (!single && k0.size(2) != T) || !head_size_ok(D) ||
+      !tables_ready(cos, sin, q0, D) || cos.requires_grad() || sin.requires_grad())
+    return not_taken();
+  if ((wq == nullptr) != (wk == nullptr)) return not_taken();
+  if (wq)
+    for (const Tensor* w : {wq, wk})
+      if (w->device() != q0.device() || w->layout() != at::kStrided || w->dim() != 1 || w->size(0) != D || w->stride(0) != 1 ||
+          w->scalar_type() != wq->scalar_type() || (w->scalar_type() != at::kFloat && w->scalar_type() != q0.scalar_type()) || !(c.eps >= 1e-30 && c.eps < INFINITY))
+        return not_taken();
+  if (pos ? !(pos->scalar_type() == at::kInt || pos->scalar_type() == at::kLong) || pos->device() != q0.device() || pos->layout() != at::kStrided ||
+                !(pos->dim() == 1 ? pos->size(0) == (single ? B : T) : pos->dim() == 2 && pos->size(0) == B && pos->size(1) == T)
+          : T > cos.size(0))
+    return not_taken();
+  if (!wq) c.eps = 1.0;   // not used
+  variable_list out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const c10::DeviceGuard guard(q0.device());
+    const Tensor q = single ? q0.unsqueeze(2) : q0, k = single ? k0.unsqueeze(2) : k0, none;
+    const Tensor positions = !pos ? none : single ? pos->unsqueeze(1) : pos->dim() == 1 ? pos->unsqueeze(0).expand({B, T}) : *pos;
+    const RotaryTables t{wq ? *wq : none, wk ? *wk : none, cos, sin, positions};
+    if (needs_grad({&q0, &k0}) || (wq && needs_grad({wq, wk}))) {
+      check_capture({&q0, &k0, wq, wk});
+      const std::optional<Tensor> w1 = wq ? std::optional<Tensor>(*wq) : std::nullopt, w2 = wk ? std::optional<Tensor>(*wk) : std::nullopt;
+      out = RotaryNode::apply(q, k, w1, w2, t, c);
+    } else {
+      out = RotaryNode::run(kernel_ready(q), kernel_ready(k), t, c);
+    }
+    if (single)
+      for (Tensor& t : out) t = t.squeeze(2);
+  }
+  PyObject* r = PyTuple_New(2);
+  if (!r) throw python_error();
+  for (int i = 0; i < 2; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(out[i]));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
 // ------------------------------------------------------------------------------------------------- module ----
 // decisions(B, H, Hk, M, N, D, num_cus, ds_limit_mib) -> every launch decision for that shape, for the test that
 // holds them against the Python functions
@@ -790,6 +1055,9 @@ PyMethodDef kMethods[] = {
     {"flash", (PyCFunction)(void*)flash, METH_FASTCALL, nullptr},
     {"piecewise", (PyCFunction)(void*)piecewise, METH_FASTCALL, nullptr},
     {"paged", (PyCFunction)(void*)paged, METH_FASTCALL, nullptr},
+    {"paged_fp8", (PyCFunction)(void*)paged_fp8, METH_FASTCALL, nullptr},
+    {"paged_append", (PyCFunction)(void*)paged_append_call, METH_FASTCALL, nullptr},
+    {"norm_rotary", (PyCFunction)(void*)norm_rotary, METH_FASTCALL, nullptr},
     {"decisions", decisions, METH_VARARGS, nullptr},
     {"forward_pieces", pieces_of_forward, METH_VARARGS, nullptr},
     {"gradient_pieces", pieces_of_gradients, METH_VARARGS, nullptr},

@@ -13,6 +13,7 @@
 
 #ifdef FLAGATTN_HOST_SIM
 #include "hw_sim.hpp"
+#include "hw_sim_e4m3.hpp"
 #else
 #include <hip/hip_runtime.h>
 
@@ -317,6 +318,27 @@ FA_DEVICE uint32_t pack2(bf16_t, float a, float b) {
   b2 v; v[0] = (__bf16)a; v[1] = (__bf16)b;
   return __builtin_bit_cast(uint32_t, v);
 }
+
+// Bytes of {a, b} picked by the four bytes of `sel`, lowest first: 0..3 are b's bytes, 4..7 a's.
+FA_DEVICE uint32_t byte_perm(uint32_t a, uint32_t b, uint32_t sel) { return __builtin_amdgcn_perm(a, b, sel); }
+// Two e4m3 codes (the low or the high half of `codes`) as packed T: every e4m3 number is one of either type.
+template <bool HIGH> FA_DEVICE uint32_t from_e4m3(half_t, uint32_t codes) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, HIGH));
+}
+template <bool HIGH> FA_DEVICE uint32_t from_e4m3(bf16_t, uint32_t codes) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, 1.0f, HIGH));
+}
+// The four codes as fp32.
+FA_DEVICE f32x4 from_e4m3(uint32_t codes) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+  return f32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+// Four fp32 values of magnitude up to 448 (or NaN) rounded to e4m3 codes, ties to even.
+FA_DEVICE uint32_t to_e4m3(f32x4 x) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
+}
+FA_DEVICE float rsqrt_fast(float x) { return __builtin_amdgcn_rsqf(x); }
 
 }  // namespace hw
 #include "pinned_regs.hpp"

@@ -132,7 +132,54 @@ struct PagedParams {
   int dtype;
   // balanced launch only: partial results of workgroups that share a (sequence, kv head) pair
   float* ws; int num_wgs;
+  // caches of e4m3 codes only: scales (num_blocks, Hkv), and the extents that block numbers are held to
+  const float *k_scales, *v_scales; int64_t scale_sblk, scale_sh;
+  int num_blocks, bt_cols;
 };
+int run_paged_e4m3(const PagedParams& p, hipStream_t stream);
+
+// Norm and rotation of queries (side 0) and keys (side 1), views of (B, heads, T, D).
+struct RotarySide {
+  View4 x, dy;             // input (the backward reads it with weights only); gradient of the output (backward)
+  View4 y;                 // written: output, or the gradient of the input
+  const void* w;           // weight (D), or null: no norm
+  void* dw;                // written by the backward where there is a weight
+  int heads;
+  int chunks, workgroups;  // filled in at the launch
+};
+struct RotaryParams {
+  RotarySide side[2];
+  const float *cos, *sin;  // (table_rows, rotary / 2), rows table_stride apart
+  int64_t table_stride, table_rows;
+  const void* positions;   // (B, T) int32 or int64 by strides, or null: a token's index
+  int pos64;
+  int64_t pos_sb, pos_st;
+  float* partial;          // backward with weights: a row of D floats per workgroup
+  float eps;
+  int B, T, D, rotary, interleaved, w_f32, dtype;
+  int heads_per_item;      // filled in at the launch
+};
+
+// Appending rows of keys (side 0) and values (side 1) to a paged cache.
+struct AppendSide {
+  const void* x; int64_t x_row, x_head;   // (rows, Hkv, D)
+  void* cache;                            // (num_blocks, Hkv, block_size, D)
+  float* scale;                           // (num_blocks, Hkv) for e4m3 codes, null for a cache of the rows' type
+};
+struct AppendParams {
+  AppendSide side[2];
+  int64_t c_blk, c_head, c_tok;           // element strides of both caches
+  int64_t s_blk, s_head;                  // and of both scales
+  const int32_t* lens;                    // (num_seqs) tokens of each sequence, the new ones counted
+  const int32_t* starts;                  // (num_seqs + 1) first row of each sequence; null: one row each
+  const void* block_tables; int bt64; int64_t bt_stride; int bt_cols;
+  const float *cos, *sin; int64_t table_stride, table_rows;
+  int64_t rows;
+  int num_blocks, num_seqs, Hkv, D, block_size;
+  int rotary, interleaved, dtype;         // rotary 0: no rotation
+  int heads_per_item;                     // filled in at the launch
+};
+int run_append(const AppendParams& p, hipStream_t stream);
 
 struct MaskParams {
   uint8_t* mask;   // (B, H, M, N) contiguous, one byte per element: 1 = kept
@@ -167,6 +214,9 @@ int run_bwd_dkdv_ds(const BwdParams& p, bool piecewise, hipStream_t stream);
 int run_bwd_dq_from_ds(const BwdParams& p, bool piecewise, hipStream_t stream);
 int run_splitkv(const SplitParams& p, hipStream_t stream);
 int run_combine(const CombineParams& p, hipStream_t stream);
+int run_rotary(RotaryParams p, hipStream_t stream);
+int run_rotary_bwd(RotaryParams p, hipStream_t stream);
+int64_t rotary_workspace_bytes(int D);   // of the backward with weights, on the current device
 int run_paged(const PagedParams& p, hipStream_t stream);
 int run_paged_reduce(const PagedParams& p, hipStream_t stream);
 int64_t paged_balanced_workspace_bytes(int num_wgs, int D);

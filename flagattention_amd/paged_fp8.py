@@ -1,0 +1,94 @@
+"""``paged_attention_fp8``: single-token decode over a paged cache of e4m3 codes with a scale for each block and kv head.
+
+No counterpart in the reference; it stands beside ``paged_attention`` and takes its arguments, with the scales behind the
+caches.  ``paged_append`` fills such a cache.
+"""
+import torch
+
+from . import _abi, _lib
+from .paged import _HEAD_SIZES, _num_cus, choose_launch
+
+__all__ = ["attention"]
+
+
+def check_cache(key_cache, value_cache, key_scales, value_scales):
+    """A pair of e4m3 caches (num_blocks, heads_kv, block_size, head_size) and their scales."""
+    assert key_cache.dtype == value_cache.dtype == torch.float8_e4m3fn, \
+        f"an 8-bit cache holds float8_e4m3fn, got {key_cache.dtype} and {value_cache.dtype}"
+    assert key_scales.dtype == value_scales.dtype == torch.float32, "the scales of an 8-bit cache are float32"
+    assert key_scales.shape == value_scales.shape == key_cache.shape[:2], \
+        f"one scale per block and kv head: got {tuple(key_scales.shape)} for a cache of {tuple(key_cache.shape)}"
+    assert key_scales.stride() == value_scales.stride(), "key and value scales must share their strides"
+
+
+def check_cache_layout(key_cache, value_cache):
+    assert key_cache.dim() == 4 and value_cache.shape == key_cache.shape
+    assert key_cache.stride() == value_cache.stride(), "key and value cache must share their strides"
+    align = 16 // key_cache.element_size()
+    assert key_cache.stride(3) == 1 and not any(s % align for n, s in zip(key_cache.shape[:3], key_cache.stride()[:3]) if n > 1) \
+        and key_cache.data_ptr() % 16 == 0 and value_cache.data_ptr() % 16 == 0, \
+        "cache rows must be 16-byte aligned, with unit stride on the last dimension"
+
+
+def check_integers(name, t, device, shape):
+    assert not t.dtype.is_floating_point and t.dtype not in (torch.bool,), f"{name} must hold integers, got {t.dtype}"
+    assert t.device == device, f"{name} must be on {device}, got {t.device}"
+    assert t.shape == shape, f"{name} must be {tuple(shape)}, got {tuple(t.shape)}"
+
+
+def int32(t):
+    """Contiguous 32-bit integers, as the kernels read them."""
+    return (t if t.dtype == torch.int32 else t.to(torch.int32)).contiguous()
+
+
+def table_ready(block_tables):
+    assert block_tables.dim() == 2 and block_tables.dtype in (torch.int32, torch.int64), "block_tables: two dimensions, int32 or int64"
+    return block_tables if block_tables.stride(1) == 1 else block_tables.contiguous()
+
+
+def attention(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables, attn_scale,
+              max_context_len):
+    """query (num_seqs, heads_q, head_size), float16 or bfloat16; key_cache / value_cache (num_blocks, heads_kv, block_size,
+    head_size), float8_e4m3fn with identical strides; key_scales / value_scales (num_blocks, heads_kv), float32: a code c
+    stands for ``c * scale``.  context_lens (num_seqs,) of any integer type; block_tables (num_seqs, max_blocks_per_seq)
+    int32 or int64; max_context_len bounds the context lengths (it decides how the work is dealt out, not what is read).
+
+    Returns out shaped like ``query``; a sequence of context length 0 gets a zero row, and so does every one where the
+    cache or the table is empty.  A key whose block number is not one of the cache's, or whose column is not in the table,
+    makes the rows that see it NaN; nothing is read for it.  Not differentiable."""
+    if query.is_cuda:   # native host path (``csrc/host.cpp``); what it does not take is served below
+        out = _lib.native().paged_fp8(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables,
+                                      attn_scale, max_context_len)
+        if out is not NotImplemented:
+            return out
+    num_seqs, num_q_heads, head_size = query.shape
+    check_cache(key_cache, value_cache, key_scales, value_scales)
+    check_cache_layout(key_cache, value_cache)
+    num_blocks, num_kv_heads, block_size, _ = key_cache.shape
+    assert key_cache.shape[3] == head_size
+    assert head_size in _HEAD_SIZES, f"head_size={head_size}"
+    assert num_kv_heads > 0 and num_q_heads % num_kv_heads == 0
+    assert all(t.device == query.device for t in (key_cache, value_cache, key_scales, value_scales, block_tables)), \
+        "all tensors must be on one device"
+    check_integers("context_lens", context_lens, query.device, (num_seqs,))
+    block_tables = table_ready(block_tables)
+    assert block_tables.shape[0] == num_seqs
+    _abi.dtype_code(query)   # raises for other types
+    if query.numel() == 0 or num_blocks == 0 or block_size == 0 or block_tables.shape[1] == 0:   # nothing to launch
+        return torch.zeros_like(query)
+    lib = _lib.get()
+    query = _abi.kernel_ready(query)
+    context_lens = int32(context_lens)
+    out = torch.empty_like(query)
+    if not _abi.is_kernel_ready(out):
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    with torch.cuda.device(query.device):
+        kind, num_wgs = choose_launch(num_seqs, num_kv_heads, num_q_heads // num_kv_heads, head_size, max_context_len,
+                                      _num_cus(lib, query.device))
+        workspace = None
+        if kind == "balanced":
+            nbytes = lib.paged_attn_balanced_workspace(num_wgs, head_size)
+            workspace = torch.empty(nbytes // 4, dtype=torch.float32, device=query.device)
+        _abi.paged_attn_e4m3(lib, out, query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables,
+                             attn_scale, workspace, num_wgs)
+    return out

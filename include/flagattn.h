@@ -284,6 +284,68 @@ int paged_attn_balanced_static(int dtype, void* out, int64_t o_stride_s, int64_t
                                int num_q_heads, int num_kv_heads, int head_size, int block_size,
                                int num_workgroups, void* stream);
 
+/* -------------------------------------------------------------- around the paged cache (no counterpart in the reference) --
+ * paged_attn_e4m3: paged_attn / paged_attn_balanced over a cache of e4m3 codes.  A code c of block b and kv head h stands for
+ * c * key_scales[b, h] (value_scales[b, h]); the scales are fp32, (num_blocks, Hkv) with the element strides
+ * scale_stride_{blk,h} for both.  Cache strides in codes, multiples of 16, caches 16-byte aligned.  dtype is that of query
+ * and out.  context_lens, block_tables, head_size as for paged_attn; bt_cols columns of the block table and num_blocks
+ * blocks exist: a key whose block number is not in 0 .. num_blocks - 1, or whose column is not in the table, makes the rows
+ * that see it NaN and nothing is read for it.  num_workgroups > 0: the balanced launch, with a workspace of
+ * paged_attn_balanced_workspace(num_workgroups, head_size) bytes; 0: one workgroup per sequence, kv head and 16 query heads,
+ * no workspace. */
+int paged_attn_e4m3(int dtype, void* out, int64_t o_stride_s, int64_t o_stride_h, const void* query,
+                    int64_t q_stride_s, int64_t q_stride_h, const void* key_cache, const void* value_cache,
+                    int64_t kv_stride_blk, int64_t kv_stride_h, int64_t kv_stride_tok, const float* key_scales,
+                    const float* value_scales, int64_t scale_stride_blk, int64_t scale_stride_h,
+                    const int32_t* context_lens, const void* block_tables, int bt_is_int64, int64_t bt_stride,
+                    int bt_cols, int num_blocks, float attn_scale, int num_seqs, int num_q_heads, int num_kv_heads,
+                    int head_size, int block_size, void* workspace, int64_t workspace_bytes, int num_workgroups,
+                    void* stream);
+
+/* paged_append: stores rows of keys and values, (rows, Hkv, D) of `dtype` with element strides *_stride_{r,h} (multiples of
+ * 8, 16-byte aligned), in a paged cache.  Sequence s has the rows starts[s] .. starts[s + 1] - 1 (starts null: row s, and
+ * rows == num_seqs); the last of them is stored at position context_lens[s] - 1, the lengths counting the new tokens.  Rows
+ * of negative position, outside 0 .. rows - 1, behind the last start, behind the block table's bt_cols columns, with a block
+ * number outside 0 .. num_blocks - 1, or (with rotation) behind the tables are not stored.  The blocks that a call stores to
+ * belong to one sequence each.
+ * Caches (num_blocks, Hkv, block_size, D), both with the element strides kv_stride_*: of `dtype` where the scales are null
+ * (strides multiples of 8), else e4m3 codes (multiples of 16) with fp32 scales (num_blocks, Hkv).  With `peak` the largest
+ * finite magnitude stored in a block and head by the call: needed = the least power of two with peak / needed <= 448, within
+ * 2^-118 .. 2^120; the scale becomes needed where the block held none of the sequence's tokens, else max(scale, needed),
+ * and where it grows the codes that are there are rounded again.  Values that are not finite become NaN.
+ * rotary_size > 0 (a multiple of 16, at most D): the first rotary_size values of a key are turned by the angles of its
+ * position, row `position` of cos / sin, (table_rows, rotary_size / 2) fp32 with rows table_stride apart (a multiple of 4,
+ * 16-byte aligned), in pairs (i, i + rotary_size / 2) or, interleaved, (2i, 2i + 1). */
+int paged_append(int dtype, const void* key, int64_t k_stride_r, int64_t k_stride_h, const void* value,
+                 int64_t v_stride_r, int64_t v_stride_h, void* key_cache, void* value_cache, int64_t kv_stride_blk,
+                 int64_t kv_stride_h, int64_t kv_stride_tok, float* key_scales, float* value_scales,
+                 int64_t scale_stride_blk, int64_t scale_stride_h, const int32_t* context_lens, const int32_t* starts,
+                 const void* block_tables, int bt_is_int64, int64_t bt_stride, int bt_cols, int num_blocks,
+                 const float* cos, const float* sin, int64_t table_stride, int64_t table_rows, int rotary_size,
+                 int interleaved, int64_t rows, int num_seqs, int num_kv_heads, int head_size, int block_size,
+                 void* stream);
+
+/* fa_norm_rotary: of every row x of q (B, H, T, D) and k (B, Hk, T, D), n = x * rsqrt(mean(x^2) + eps) * weight (weights
+ * null: n = x), turned as by paged_append at the row's position: positions[b, t] (int32 or int64, element strides
+ * pos_stride_*), or t where positions is null.  A position without a row in the tables turns by NaN.  Weights (D) of
+ * `dtype`, or fp32 with weights_f32; both or neither.  eps > 0.  D in {16, 32, 64, 128, 256, 512}.
+ * fa_norm_rotary_bwd: gradients of q and k (and of the weights, in the weights' type) from those of the outputs.  With
+ * weights the workspace holds at least fa_norm_rotary_workspace(D) bytes, 16-byte aligned, contents irrelevant; without,
+ * q, k and the workspace are not read and may be null.  Sums are formed in an order that depends on the sizes alone. */
+int fa_norm_rotary(int dtype, const fa_view4* q, const fa_view4* k, const fa_view4* q_out, const fa_view4* k_out,
+                   const void* q_weight, const void* k_weight, int weights_f32, const float* cos, const float* sin,
+                   int64_t table_stride, int64_t table_rows, int rotary_size, int interleaved, const void* positions,
+                   int positions_int64, int64_t pos_stride_b, int64_t pos_stride_t, float eps, int B, int H, int Hk,
+                   int T, int D, void* stream);
+int fa_norm_rotary_workspace(int D);
+int fa_norm_rotary_bwd(int dtype, const fa_view4* q, const fa_view4* k, const fa_view4* dq_out, const fa_view4* dk_out,
+                       const fa_view4* dq, const fa_view4* dk, const void* q_weight, const void* k_weight,
+                       void* dq_weight, void* dk_weight, int weights_f32, const float* cos, const float* sin,
+                       int64_t table_stride, int64_t table_rows, int rotary_size, int interleaved,
+                       const void* positions, int positions_int64, int64_t pos_stride_b, int64_t pos_stride_t,
+                       float eps, int B, int H, int Hk, int T, int D, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+
 /* fa_probe_mfma: a measurement aid, no counterpart in the reference.  Enqueues one workgroup per compute unit
  * (fa_num_cus() of them, 256 threads each, one wavefront per SIMD) whose wavefronts issue nothing but
  * iters * 16 32x32x16 matrix instructions of the given dtype from registers: 2 * 32 * 32 * 16 FLOP each, so the

@@ -27,7 +27,11 @@ randomized three-way comparison), see ``tests/test_oracle_*.py``:
   rate, Triton's ``tl.rand`` and the reference's recomputed masks bit for bit; dropout with an all-true
   mask equals no dropout; a hand-built mask against an explicit loop.
 
-All three operators are also held against fixed vectors (``tests/golden/attention_vectors.npz``, written by
+* ``rotary`` and ``paged_cache`` state operators that the reference does not have, in 64 bits: turns as complex products,
+  gradients against differences, e4m3 rounding against torch's conversion, the 8-bit cache against dense attention over the
+  values it stands for (``tests/test_oracle_cache.py``).
+
+All three operators of the reference are also held against fixed vectors (``tests/golden/attention_vectors.npz``, written by
 ``tests/golden/make_vectors.py`` from scalar fp64 loops that state the definitions directly): bottom-right
 causal alignment with grouped heads, rows without keys, the piecewise distance rule, the paged block
 table (``tests/test_golden.py``; the same vectors check the kernels in the simulator and on the GPU).
@@ -41,3 +45,4 @@ from .piecewise import piecewise_attention, piecewise_attention_grad  # noqa: F4
 from .paged import paged_attention  # noqa: F401
 from .compare import max_abs_diff, within_two_x  # noqa: F401
 from .dropout import keep_mask  # noqa: F401
+from . import paged_cache, rotary  # noqa: F401
