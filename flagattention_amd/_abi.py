@@ -323,7 +323,7 @@ def paged_attn_e4m3(lib, out, query, key_cache, value_cache, key_scales, value_s
     """workspace None and num_workgroups 0: one workgroup per sequence, kv head and 16 query heads."""
     num_seqs, Hq, D = query.shape
     num_blocks, Hkv, block_size, _ = key_cache.shape
-    check(lib.paged_attn_e4m3(dtype_code(query), ptr(out), out.stride(0), out.stride(1),
+    check(lib.paged_attn_e4m3(dtype_code(query), ptr(out), used_stride(out, 0), used_stride(out, 1),
                               ptr(query), used_stride(query, 0), used_stride(query, 1), ptr(key_cache), ptr(value_cache),
                               used_stride(key_cache, 0), used_stride(key_cache, 1), used_stride(key_cache, 2),
                               ptr(key_scales), ptr(value_scales), key_scales.stride(0), key_scales.stride(1),

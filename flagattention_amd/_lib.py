@@ -54,6 +54,7 @@ SIGNATURES = {
     "paged_attn_balanced_workspace": [_i, _i],
     "paged_attn_balanced": [_i, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i, _i64,
                             _f, _i, _i, _i, _i, _i, _p, _i64, _i, _p],
+    "paged_attn_e4m3_workspace": [_i, _i],
     "paged_attn_e4m3": [_i, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i, _i64,
                         _i, _i, _f, _i, _i, _i, _i, _i, _p, _i64, _i, _p],
     "paged_append": [_i, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _p, _i, _i64,

@@ -54,7 +54,8 @@ def append(key, value, key_cache, value_cache, context_lens, block_tables, query
     _abi.dtype_code(key)   # raises for other types
     check_cache_layout(key_cache, value_cache)
     num_blocks, _, block_size, _ = key_cache.shape
-    assert key_cache.shape[1] == num_kv_heads and key_cache.shape[3] == head_size
+    assert key_cache.shape[1] == num_kv_heads and key_cache.shape[3] == head_size, \
+        f"rows of {num_kv_heads} heads of {head_size}, and a cache of {tuple(key_cache.shape)}"
     assert head_size in _HEAD_SIZES, f"head_size={head_size}"
     assert (key_scales is None) == (value_scales is None), "key_scales and value_scales: both or neither"
     tensors = [value, key_cache, value_cache, block_tables]

@@ -524,6 +524,11 @@ int paged_attn_balanced_static(int dtype, void* out, int64_t o_stride_s, int64_t
 
 static bool paged_head_size_ok(int D) { return D == 16 || D == 32 || D == 64 || D == 128 || D == 256 || D == 512; }
 
+int paged_attn_e4m3_workspace(int num_workgroups, int head_size) {
+  if (num_workgroups <= 0 || num_workgroups > 0x7fffffff / 4) return FA_ERR_BAD_ARGUMENT;
+  return paged_attn_balanced_workspace(4 * num_workgroups, head_size);   // for every wavefront what that has for a workgroup
+}
+
 int paged_attn_e4m3(int dtype, void* out, int64_t o_stride_s, int64_t o_stride_h, const void* query,
                     int64_t q_stride_s, int64_t q_stride_h, const void* key_cache, const void* value_cache,
                     int64_t kv_stride_blk, int64_t kv_stride_h, int64_t kv_stride_tok, const float* key_scales,
@@ -537,12 +542,14 @@ int paged_attn_e4m3(int dtype, void* out, int64_t o_stride_s, int64_t o_stride_h
                             num_kv_heads, head_size, 0, 1, nullptr, nullptr, nullptr);
   if (rc) return rc;
   if (!query || !key_cache || !value_cache || !block_tables || !key_scales || !value_scales) return FA_ERR_BAD_ARGUMENT;
-  if ((((uintptr_t)query) | ((uintptr_t)key_cache) | ((uintptr_t)value_cache) | ((uintptr_t)workspace)) & 15) return FA_ERR_BAD_ARGUMENT;
+  if ((((uintptr_t)query) | ((uintptr_t)key_cache) | ((uintptr_t)value_cache) | ((uintptr_t)workspace) | ((uintptr_t)out)) & 15)
+    return FA_ERR_BAD_ARGUMENT;
   if ((((uintptr_t)key_scales) | ((uintptr_t)value_scales)) & 3) return FA_ERR_BAD_ARGUMENT;
-  if ((q_stride_s | q_stride_h) % 8 || (kv_stride_blk | kv_stride_h | kv_stride_tok) % 16) return FA_ERR_BAD_ARGUMENT;
+  if ((q_stride_s | q_stride_h | o_stride_s | o_stride_h) % 8 || (kv_stride_blk | kv_stride_h | kv_stride_tok) % 16) return FA_ERR_BAD_ARGUMENT;
   if (!paged_head_size_ok(head_size)) return FA_ERR_UNSUPPORTED;
   if (num_workgroups < 0) return FA_ERR_BAD_ARGUMENT;
-  if (num_workgroups > 0 && (!workspace || workspace_bytes < fa::paged_balanced_workspace_bytes(num_workgroups, head_size)))
+  if (num_workgroups > 0 && (!workspace || num_workgroups > 0x7fffffff / 4 ||
+                             workspace_bytes < fa::paged_balanced_workspace_bytes(4 * num_workgroups, head_size)))
     return FA_ERR_BAD_ARGUMENT;
   p.q = query; p.q_ss = q_stride_s; p.q_sh = q_stride_h;
   p.kc = key_cache; p.vc = value_cache;

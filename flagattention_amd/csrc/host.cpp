@@ -182,6 +182,14 @@ int balanced_workgroups(int64_t seqs, int64_t Hkv, int64_t group, int64_t D, int
   return seqs * Hkv * cdiv(group, 16) >= 8 * (int64_t)wgs && max_context <= 2048 ? 0 : wgs;
 }
 
+// paged_fp8.choose_workgroups (the reasons and figures stand there)
+int e4m3_workgroups(int64_t seqs, int64_t Hkv, int64_t group, int64_t D, int64_t max_context, int cus) {
+  const double pairs = (double)(seqs * Hkv * cdiv(group, 16)), stream = pairs * (double)max_context * (double)D / 5.5e6;
+  const double step = D <= 64 ? 1.05 : D == 128 ? 1.4 : D == 256 ? 2.2 : 4.5, balanced = D <= 128 ? 9.5 : D == 256 ? 12.0 : 15.0;
+  const double alone = 3.0 + step * (double)cdiv(max_context, 128) + 0.6 * stream;
+  return alone <= balanced + stream ? 0 : cus * (D <= 64 ? 4 : D <= 256 ? 2 : 1);
+}
+
 // ------------------------------------------------------------------------------------------------ tensors ----
 int dtype_code(const Tensor& t) { return t.scalar_type() == at::kHalf ? FA_F16 : FA_BF16; }
 
@@ -809,10 +817,10 @@ PyObject* paged_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     pybind11::gil_scoped_release no_gil;
     const c10::DeviceGuard guard(q.device());
     out = empty_result(q);
-    const int wgs = balanced_workgroups(seqs, Hkv, Hq / Hkv, D, longest, fa_num_cus());
-    const int64_t bytes = wgs > 0 ? paged_attn_balanced_workspace(wgs, (int)D) : 0;
+    const int wgs = e4m3_workgroups(seqs, Hkv, Hq / Hkv, D, longest, fa_num_cus());
+    const int64_t bytes = wgs > 0 ? paged_attn_e4m3_workspace(wgs, (int)D) : 0;
     Tensor ws = wgs > 0 ? empty({bytes / 4}, at::kFloat, q) : Tensor();
-    check(paged_attn_e4m3(dtype_code(q), out.mutable_data_ptr(), out.stride(0), out.stride(1), q.const_data_ptr(), used_stride(q, 0),
+    check(paged_attn_e4m3(dtype_code(q), out.mutable_data_ptr(), used_stride(out, 0), used_stride(out, 1), q.const_data_ptr(), used_stride(q, 0),
                           used_stride(q, 1), kc.const_data_ptr(), vc.const_data_ptr(), used_stride(kc, 0), used_stride(kc, 1), used_stride(kc, 2),
                           f32(ks), f32(vs), ks.stride(0), ks.stride(1), (const int32_t*)lens.const_data_ptr(), bt.const_data_ptr(),
                           bt.scalar_type() == at::kLong, bt.stride(0), (int)bt.size(1), (int)kc.size(0), (float)scale, (int)seqs, (int)Hq,
@@ -1037,6 +1045,13 @@ PyObject* pieces_of_gradients(PyObject*, PyObject* args) {
   return Py_BuildValue("(ii)", p.kv, p.q);
 }
 
+// e4m3_workgroups(sequences, kv heads, group, D, longest, num_cus)
+PyObject* workgroups_of_e4m3(PyObject*, PyObject* args) {
+  long long seqs, Hkv, group, D, longest, cus;
+  if (!PyArg_ParseTuple(args, "LLLLLL", &seqs, &Hkv, &group, &D, &longest, &cus)) return nullptr;
+  return PyLong_FromLong(e4m3_workgroups(seqs, Hkv, group, D, longest, (int)cus));
+}
+
 // keeps_mask(N, D)
 PyObject* mask_is_kept(PyObject*, PyObject* args) {
   long long N, D;
@@ -1061,6 +1076,7 @@ PyMethodDef kMethods[] = {
     {"decisions", decisions, METH_VARARGS, nullptr},
     {"forward_pieces", pieces_of_forward, METH_VARARGS, nullptr},
     {"gradient_pieces", pieces_of_gradients, METH_VARARGS, nullptr},
+    {"e4m3_workgroups", workgroups_of_e4m3, METH_VARARGS, nullptr},
     {"keeps_mask", mask_is_kept, METH_VARARGS, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};

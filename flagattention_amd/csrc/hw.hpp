@@ -339,6 +339,10 @@ FA_DEVICE uint32_t to_e4m3(f32x4 x) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], lo, true);
 }
 FA_DEVICE float rsqrt_fast(float x) { return __builtin_amdgcn_rsqf(x); }
+// Loads and stores of data that is touched once: marked non-temporal.  Whole 128-byte lines per instruction only: a line of
+// which another instruction wants the rest may be gone by then.
+template <class V> FA_DEVICE V load_once(const void* p) { return __builtin_nontemporal_load((const V*)p); }
+template <class V> FA_DEVICE void store_once(void* p, V v) { __builtin_nontemporal_store(v, (V*)p); }
 
 }  // namespace hw
 #include "pinned_regs.hpp"

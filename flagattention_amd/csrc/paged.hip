@@ -233,7 +233,8 @@ FA_KERNEL void FA_LAUNCH_BOUNDS2(kThreads, (D <= 128 ? 2 : 1)) paged_balanced_ke
 //
 // A chain of memory latencies like fa_combine_kernel, and laid out like it: four output elements per thread, the
 // threads that the rows of the pair leave over share its partials between them, eight at a time, and meet in LDS.
-// One sequence of 16000 keys and 8 kv heads (63 partials per pair, 4 rows), both kernels: 40 -> 23 us.
+// One sequence of 16000 keys and 8 kv heads (63 partials per pair, 4 rows), both kernels: 40 -> 23 us.  Rows that do not fit
+// side by side are dealt to workgroups (grid y).
 template <class T, int D>
 FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) paged_balanced_reduce_kernel(PagedParams p) {
   FA_LDS_DECL(smem);
@@ -254,82 +255,82 @@ FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) paged_balanced_reduce_kernel(PagedPara
   float* area = (float*)smem;                      // value e of thread t at [e][t]
   const bool out_aligned = (((uintptr_t)p.out | (uintptr_t)(p.o_ss * 2) | (uintptr_t)(p.o_sh * 2)) & 7) == 0;
   constexpr int kBatch = 8;
-  for (int row0 = 0; row0 < rows; row0 += side) {
-    const int row = row0 + set % side, rc = imin(row, rows - 1);
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, z = 0.f, top = neg_inf();
-    for (int j0 = share * kBatch; j0 < n; j0 += shares * kBatch) {
-      float mv[kBatch], lv[kBatch];
-      hw::f32x4 ov[kBatch];
+  const int row0 = side * hw::block_y();   // one round of rows to a workgroup
+  if (row0 >= rows) return;
+  const int row = row0 + set % side, rc = imin(row, rows - 1);
+  float acc[4] = {0.f, 0.f, 0.f, 0.f}, z = 0.f, top = neg_inf();
+  for (int j0 = share * kBatch; j0 < n; j0 += shares * kBatch) {
+    float mv[kBatch], lv[kBatch];
+    hw::f32x4 ov[kBatch];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int j = imin(j0 + u, n - 1);
-        const float* slot = p.ws + (int64_t)(j == 0 ? 2 * w + 1 : 2 * (w + j)) * SF;
-        mv[u] = slot[16 * D + rc];
-        lv[u] = slot[16 * D + 16 + rc];
-        ov[u] = *(const hw::f32x4*)(slot + rc * D + d);
-      }
-      float t = top;
+    for (int u = 0; u < kBatch; ++u) {
+      const int j = imin(j0 + u, n - 1);
+      const float* slot = p.ws + (int64_t)(j == 0 ? 2 * w + 1 : 2 * (w + j)) * SF;
+      mv[u] = slot[16 * D + rc];
+      lv[u] = slot[16 * D + 16 + rc];
+      ov[u] = *(const hw::f32x4*)(slot + rc * D + d);
+    }
+    float t = top;
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) t = fmaxf(t, mv[u]);
-      if (t > top) {   // -inf -> weight 0
-        const float old = hw::exp2_fast((top - t) * kLog2e);
-        z *= old;
+    for (int u = 0; u < kBatch; ++u) t = fmaxf(t, mv[u]);
+    if (t > top) {   // -inf -> weight 0
+      const float old = hw::exp2_fast((top - t) * kLog2e);
+      z *= old;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] *= old;
-        top = t;
-      }
+      for (int e = 0; e < 4; ++e) acc[e] *= old;
+      top = t;
+    }
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        if (j0 + u < n && lv[u] != 0.f) {
-          const float wgt = lv[u] * hw::exp2_fast((mv[u] - top) * kLog2e);
-          z += wgt;
+    for (int u = 0; u < kBatch; ++u) {
+      if (j0 + u < n && lv[u] != 0.f) {
+        const float wgt = lv[u] * hw::exp2_fast((mv[u] - top) * kLog2e);
+        z += wgt;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] += wgt * ov[u][e];
-        }
+        for (int e = 0; e < 4; ++e) acc[e] += wgt * ov[u][e];
       }
     }
-    if (shares > 1) {   // the same branch in every thread
-      hw::block_sync();   // an earlier round has been read out
+  }
+  if (shares > 1) {   // the same branch in every thread
 #pragma unroll
-      for (int e = 0; e < 4; ++e) area[e * kThreads + tid] = acc[e];
-      area[4 * kThreads + tid] = z;
-      area[5 * kThreads + tid] = top;
-      hw::block_sync();
-      if (share == 0) {
-        for (int g = 1; g < shares; ++g) top = fmaxf(top, area[5 * kThreads + tid + g * side * kLanes]);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f}, zs = 0.f;
-        for (int g = 0; g < shares; ++g) {
-          const int at = tid + g * side * kLanes;
-          const float own = area[5 * kThreads + at];   // -inf in all shares: nothing but zeroes, or NaN, to add
-          const float wgt = own == top ? 1.f : hw::exp2_fast((own - top) * kLog2e);
-          zs += wgt * area[4 * kThreads + at];
+    for (int e = 0; e < 4; ++e) area[e * kThreads + tid] = acc[e];
+    area[4 * kThreads + tid] = z;
+    area[5 * kThreads + tid] = top;
+    hw::block_sync();
+    if (share == 0) {
+      for (int g = 1; g < shares; ++g) top = fmaxf(top, area[5 * kThreads + tid + g * side * kLanes]);
+      float sum[4] = {0.f, 0.f, 0.f, 0.f}, zs = 0.f;
+      for (int g = 0; g < shares; ++g) {
+        const int at = tid + g * side * kLanes;
+        const float own = area[5 * kThreads + at];   // -inf in all shares: nothing but zeroes, or NaN, to add
+        const float wgt = own == top ? 1.f : hw::exp2_fast((own - top) * kLog2e);
+        zs += wgt * area[4 * kThreads + at];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sum[e] += wgt * area[e * kThreads + at];
-        }
-        z = zs;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = sum[e];
+        for (int e = 0; e < 4; ++e) sum[e] += wgt * area[e * kThreads + at];
       }
+      z = zs;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = sum[e];
     }
-    if (share == 0 && row < rows) {
-      const float inv = z == 0.f ? 0.f : 1.f / z;
-      T* o = (T*)p.out + (int64_t)seq * p.o_ss + (int64_t)(hk * G + rb * 16 + row) * p.o_sh + d;
-      if (out_aligned) {
-        hw::u32x2 packed;
-        packed[0] = hw::pack2(T{}, acc[0] * inv, acc[1] * inv);
-        packed[1] = hw::pack2(T{}, acc[2] * inv, acc[3] * inv);
-        *(hw::u32x2*)o = packed;
-      } else {
+  }
+  if (share == 0 && row < rows) {
+    const float inv = z == 0.f ? 0.f : 1.f / z;
+    T* o = (T*)p.out + (int64_t)seq * p.o_ss + (int64_t)(hk * G + rb * 16 + row) * p.o_sh + d;
+    if (out_aligned) {
+      hw::u32x2 packed;
+      packed[0] = hw::pack2(T{}, acc[0] * inv, acc[1] * inv);
+      packed[1] = hw::pack2(T{}, acc[2] * inv, acc[3] * inv);
+      *(hw::u32x2*)o = packed;
+    } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (T)(acc[e] * inv);
-      }
+      for (int e = 0; e < 4; ++e) o[e] = (T)(acc[e] * inv);
     }
   }
 }
 
 template <class T>
 static int launch_balanced_reduce(const PagedParams& p, hipStream_t stream) {
-  dim3 grid(p.num_wgs, 1, 1);
+  const int group = p.Hq / p.Hkv, at_once = 1024 / p.D;   // rows of a pair, and those that a workgroup has threads for
+  dim3 grid(p.num_wgs, ((group < 16 ? group : 16) + at_once - 1) / at_once, 1);
   constexpr size_t lds = 6 * kThreads * sizeof(float);
   switch (p.D) {
     case 16: return launch(paged_balanced_reduce_kernel<T, 16>, grid, lds, stream, p);

@@ -31,12 +31,16 @@ constexpr int kMinUnitsPerWg = 2;   // where a range may cross pairs
 FA_DEVICE int balanced_slot_floats(int D) { return 16 * D + 32; }
 
 // Runs pair(seq, hk, rb, n_begin, n_end, whole, slot index) for every piece of a pair in this workgroup's range, and clears
-// the output rows of empty sequences.  STEP_KEYS: the keys of a wavefront's step.
-template <class T, int STEP_KEYS, class Pair>
+// the output rows of empty sequences.  STEP_KEYS: the keys of a wavefront's step.  WAVES: every wavefront has a range of its
+// own, in units of one step (the workgroups above are wavefronts then, four times as many), and pieces are dealt so however
+// few pairs there are.
+template <class T, int STEP_KEYS, bool WAVES = false, class Pair>
 FA_DEVICE void balanced_walk(const PagedParams& p, const int D, Pair pair) {
-  constexpr int kUnitKeys = 4 * STEP_KEYS, kStepKeys = STEP_KEYS;
-  const int tid = hw::thread_id(), lane = tid & 63;
-  const int w = hw::block_x();
+  constexpr int kUnitKeys = WAVES ? STEP_KEYS : 4 * STEP_KEYS, kStepKeys = STEP_KEYS;
+  constexpr int kMembers = WAVES ? 64 : kThreads;
+  const int lane = hw::thread_id() & 63, tid = WAVES ? lane : hw::thread_id();
+  const int w = WAVES ? hw::uniform(4 * hw::block_x() + (hw::thread_id() >> 6)) : hw::block_x();
+  const int num_wgs = WAVES ? 4 * p.num_wgs : p.num_wgs;
   const int G = p.Hq / p.Hkv;
   const int row_blocks = (G + 15) / 16;
   const int pairs_per_seq = p.Hkv * row_blocks;
@@ -45,7 +49,7 @@ FA_DEVICE void balanced_walk(const PagedParams& p, const int D, Pair pair) {
   auto length_of = [&](int s) { return s < p.num_seqs ? imax(0, p.context_lens[s]) : 0; };
   const int first_lengths = length_of(lane);   // both scans begin with these
   const int64_t num_pairs = (int64_t)p.num_seqs * pairs_per_seq;
-  const bool one_each = 4 * num_pairs <= p.num_wgs;
+  const bool one_each = !WAVES && 4 * num_pairs <= num_wgs;
   const int grain = one_each ? kStepKeys : kUnitKeys;
   int total_units = 0;
   for (int base = 0; base < p.num_seqs; base += 64) {
@@ -54,28 +58,28 @@ FA_DEVICE void balanced_walk(const PagedParams& p, const int D, Pair pair) {
     // An empty sequence has no keys to stream: its output rows are zero.  Every wavefront sees the same
     // empty sequences here; they are dealt round-robin to the workgroups, and the threads of the one
     // that takes a sequence clear its rows together.
-    for (uint64_t todo = hw::ballot(s < p.num_seqs && u == 0 && s % p.num_wgs == w); todo; todo &= todo - 1) {
+    for (uint64_t todo = hw::ballot(s < p.num_seqs && u == 0 && s % num_wgs == w); todo; todo &= todo - 1) {
       const int e = base + __builtin_ctzll(todo);
-      for (int i = tid; i < p.Hq * D; i += kThreads) ((T*)p.out)[(int64_t)e * p.o_ss + (int64_t)(i / D) * p.o_sh + i % D] = (T)0.f;
+      for (int i = tid; i < p.Hq * D; i += kMembers) ((T*)p.out)[(int64_t)e * p.o_ss + (int64_t)(i / D) * p.o_sh + i % D] = (T)0.f;
     }
     total_units += hw::last_lane(hw::wave_prefix_sum(u));
   }
   // everything derived from the total (the key ranges, the step counts of the wavefronts) stays in scalar registers
   const int64_t total0 = (int64_t)total_units * pairs_per_seq;
-  const int64_t per = one_each ? 1 : (int64_t)imax(kMinUnitsPerWg, (int)((total0 + p.num_wgs - 1) / p.num_wgs));
+  const int64_t per = one_each ? 1 : (int64_t)imax(kMinUnitsPerWg, (int)((total0 + num_wgs - 1) / num_wgs));
   int unit_keys = kUnitKeys;
   if (one_each) {
     // Pieces of n steps' worth of keys: sum over pairs of ceil(steps / n) is at most total / n + pairs, and about
     // total / n + pairs / 2.  The n that makes the latter num_wgs is taken if the pieces really fit, else the safe one.
     auto steps_for = [&](int64_t wgs) { return (int)imax(kUnitKeys / kStepKeys, (int)((total0 + wgs - 1) / wgs)); };
-    const int tight = steps_for(p.num_wgs - num_pairs / 2);
+    const int tight = steps_for(num_wgs - num_pairs / 2);
     int pieces = 0;
     for (int base = 0; base < p.num_seqs; base += 64)
       pieces += hw::last_lane(hw::wave_prefix_sum(cdiv(base == 0 ? first_lengths : length_of(base + lane), tight * kStepKeys)));
-    unit_keys = kStepKeys * ((int64_t)pieces * pairs_per_seq <= p.num_wgs ? tight : steps_for(p.num_wgs - num_pairs));
+    unit_keys = kStepKeys * ((int64_t)pieces * pairs_per_seq <= num_wgs ? tight : steps_for(num_wgs - num_pairs));
   }
   const int64_t u_begin = (int64_t)w * per;
-  int* meta = (int*)(p.ws + (int64_t)2 * p.num_wgs * balanced_slot_floats(D)) + 4 * w;
+  int* meta = (int*)(p.ws + (int64_t)2 * num_wgs * balanced_slot_floats(D)) + 4 * w;
   // the sequence whose pairs hold unit u_begin, and the units of the sequences before it
   int seq = 0, before = 0, all_units = 0;
   {

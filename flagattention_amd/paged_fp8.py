@@ -6,9 +6,31 @@ caches.  ``paged_append`` fills such a cache.
 import torch
 
 from . import _abi, _lib
-from .paged import _HEAD_SIZES, _num_cus, choose_launch
+from .paged import _HEAD_SIZES, _num_cus
 
 __all__ = ["attention"]
+
+
+# By head size: microseconds that a workgroup alone on its pair takes for 128 keys (four wavefronts, a step each), and that a
+# balanced launch takes before it streams (two kernels, the scan of the context lengths, the merge).
+_STEP_US = {16: 1.05, 32: 1.05, 64: 1.05, 128: 1.4, 256: 2.2, 512: 4.5}
+_BALANCED_US = {16: 9.5, 32: 9.5, 64: 9.5, 128: 9.5, 256: 12.0, 512: 15.0}
+
+
+def choose_workgroups(num_seqs, num_kv_heads, group, head_size, max_context_len, num_cus):
+    """Workgroups of the balanced launch, or 0 for one workgroup per (sequence, kv head, 16 query heads), a single kernel
+    that the hardware deals out by itself.  That is as long as the longest sequence takes one workgroup and, with many pairs,
+    as the keys' bytes take at 5.5 TB/s, of which the part behind the longest one counts.  Lengths are taken to be spread up
+    to the longest.  Measured, one per pair against balanced (us, lengths uniform up to the longest, D = 128):
+    8 pairs of up to 512 keys 8.6 / 9.8, of 1024 13.4 / 10.3; 512 pairs of 1024 22 / 28, of 2048 39.5 / 39.6, of 4096 74 / 66;
+    2048 pairs of 2048 104 / 117; D = 64: 4096 pairs of 1024 61 / 74; D = 256: 4 pairs of 256 9.4 / 12.0, of 512 14 / 12.
+    A compute unit holds four workgroups up to head size 64, two up to 256 and one above."""
+    pairs = num_seqs * num_kv_heads * (-(-group // 16))
+    stream = pairs * max_context_len * head_size / 5.5e6
+    alone = 3.0 + _STEP_US[head_size] * (-(-max_context_len // 128)) + 0.6 * stream
+    if alone <= _BALANCED_US[head_size] + stream:
+        return 0
+    return num_cus * (4 if head_size <= 64 else 2 if head_size <= 256 else 1)
 
 
 def check_cache(key_cache, value_cache, key_scales, value_scales):
@@ -65,7 +87,7 @@ def attention(query, key_cache, value_cache, key_scales, value_scales, context_l
     check_cache(key_cache, value_cache, key_scales, value_scales)
     check_cache_layout(key_cache, value_cache)
     num_blocks, num_kv_heads, block_size, _ = key_cache.shape
-    assert key_cache.shape[3] == head_size
+    assert key_cache.shape[3] == head_size, f"head_size={head_size}, and a cache of {key_cache.shape[3]}"
     assert head_size in _HEAD_SIZES, f"head_size={head_size}"
     assert num_kv_heads > 0 and num_q_heads % num_kv_heads == 0
     assert all(t.device == query.device for t in (key_cache, value_cache, key_scales, value_scales, block_tables)), \
@@ -83,11 +105,11 @@ def attention(query, key_cache, value_cache, key_scales, value_scales, context_l
     if not _abi.is_kernel_ready(out):
         out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
     with torch.cuda.device(query.device):
-        kind, num_wgs = choose_launch(num_seqs, num_kv_heads, num_q_heads // num_kv_heads, head_size, max_context_len,
-                                      _num_cus(lib, query.device))
+        num_wgs = choose_workgroups(num_seqs, num_kv_heads, num_q_heads // num_kv_heads, head_size, int(max_context_len),
+                                    _num_cus(lib, query.device))
         workspace = None
-        if kind == "balanced":
-            nbytes = lib.paged_attn_balanced_workspace(num_wgs, head_size)
+        if num_wgs > 0:
+            nbytes = lib.paged_attn_e4m3_workspace(num_wgs, head_size)
             workspace = torch.empty(nbytes // 4, dtype=torch.float32, device=query.device)
         _abi.paged_attn_e4m3(lib, out, query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables,
                              attn_scale, workspace, num_wgs)

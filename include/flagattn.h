@@ -290,9 +290,10 @@ int paged_attn_balanced_static(int dtype, void* out, int64_t o_stride_s, int64_t
  * scale_stride_{blk,h} for both.  Cache strides in codes, multiples of 16, caches 16-byte aligned.  dtype is that of query
  * and out.  context_lens, block_tables, head_size as for paged_attn; bt_cols columns of the block table and num_blocks
  * blocks exist: a key whose block number is not in 0 .. num_blocks - 1, or whose column is not in the table, makes the rows
- * that see it NaN and nothing is read for it.  num_workgroups > 0: the balanced launch, with a workspace of
- * paged_attn_balanced_workspace(num_workgroups, head_size) bytes; 0: one workgroup per sequence, kv head and 16 query heads,
- * no workspace. */
+ * that see it NaN and nothing is read for it.  out and its strides are aligned as query and its.  num_workgroups > 0: the
+ * balanced launch, with a workspace of paged_attn_e4m3_workspace(num_workgroups, head_size) bytes (at most INT_MAX), 16-byte
+ * aligned, contents irrelevant; 0: one workgroup per sequence, kv head and 16 query heads, no workspace. */
+int paged_attn_e4m3_workspace(int num_workgroups, int head_size);
 int paged_attn_e4m3(int dtype, void* out, int64_t o_stride_s, int64_t o_stride_h, const void* query,
                     int64_t q_stride_s, int64_t q_stride_h, const void* key_cache, const void* value_cache,
                     int64_t kv_stride_blk, int64_t kv_stride_h, int64_t kv_stride_tok, const float* key_scales,

@@ -48,6 +48,8 @@ inline uint32_t to_e4m3(f32x4 x) {
   for (int i = 0; i < 4; ++i) r |= (uint32_t)e4m3_code(x[i]) << (8 * i);
   return r;
 }
+template <class V> inline V load_once(const void* p) { return *(const V*)p; }
+template <class V> inline void store_once(void* p, V v) { *(V*)p = v; }
 inline float rsqrt_fast(float x) { return 1.f / sqrtf(x); }
 
 }  // namespace hw

@@ -45,7 +45,7 @@ def test_attention_cut_over_workgroups_and_one_workgroup_per_pair(simulator_behi
     q, *rest, longest = args
     for wgs in (0, 3, 16):
         out = torch.full_like(q, torch.nan)
-        ws = torch.empty(lib.paged_attn_balanced_workspace(max(1, wgs), 64) // 4) if wgs else None
+        ws = torch.empty(lib.paged_attn_e4m3_workspace(max(1, wgs), 64) // 4) if wgs else None
         _abi.paged_attn_e4m3(lib, out, q, *rest, ws, wgs)
         cases.check_attention(args, out, f"{wgs} workgroups")
 
