@@ -14,7 +14,7 @@
 //
 // Bound by memory (each new value is read and stored once) or, for single tokens, by the chain length -> table -> scale ->
 // store.  A wavefront of the 16-bit kernel holds 1024 / D rows and walks a run of heads; one of the 8-bit kernel has one
-// block of one head, of the keys or of the values, so that the scale is its own.
+// block of one head, keys and values, so that the scales are its own.
 #include "rotary.hpp"
 
 namespace fa {
@@ -31,16 +31,20 @@ FA_DEVICE NewRows new_rows(const AppendParams& p, int s) {
   const int64_t next = p.starts[s + 1], b = clamp64(p.starts[s], 0, p.rows);
   return NewRows{b, clamp64(next, b, p.rows), ctx - next};
 }
-// The last sequence s with key(s) <= x (keys do not fall; -1 if there is none).
+// The last of n sequences with key(s) <= x (keys do not fall; -1 if there is none), found by the wavefront together: 64 at a
+// time, so that up to 64 sequences take one load's latency, up to 4160 two.
 template <class Key>
-FA_DEVICE int last_not_above(int n, int64_t x, Key key) {
-  int lo = -1, hi = n;   // key(lo) <= x < key(hi)
-  while (hi - lo > 1) {
-    const int mid = lo + (hi - lo) / 2;
-    if (key(mid) <= x) lo = mid;
-    else hi = mid;
+FA_DEVICE int last_not_above(int n, int64_t x, int lane, Key key) {
+  int base = 0, found = -1;
+  while (base < n) {
+    const int step = (n - base + 63) / 64, i = base + lane * step;
+    const int count = __builtin_popcountll(hw::ballot(i < n && key(imin(i, n - 1)) <= x));
+    if (count == 0) break;
+    found = base + (count - 1) * step;
+    n = imin(n, found + step);
+    base = found + 1;
   }
-  return lo;
+  return hw::uniform(found);
 }
 // positions that have a place
 FA_DEVICE int64_t position_limit(const AppendParams& p) {
@@ -52,43 +56,55 @@ FA_DEVICE int64_t block_of_table(const AppendParams& p, int s, int64_t column) {
   return p.bt64 ? ((const int64_t*)p.block_tables)[at] : ((const int32_t*)p.block_tables)[at];
 }
 
+template <class T>
+FA_DEVICE void store_raw(T* row, RotaryPlace at, const RawRow& r) {
+  *(u32x4*)(row + at.lo) = r.lo;
+  *(u32x4*)(row + at.hi) = r.hi;
+}
+
 template <class T, int D, bool INTER>
 FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) append_kernel(AppendParams p) {
   const int lane = hw::thread_id() & 63;
   const int item = hw::uniform(hw::block_x() * kAppendWaves + (hw::thread_id() >> 6));
   const int chunks = (p.Hkv + p.heads_per_item - 1) / p.heads_per_item;
   const int h0 = item % chunks * p.heads_per_item, h1 = imin(h0 + p.heads_per_item, p.Hkv);
-  const int64_t row = (int64_t)(item / chunks) * (1024 / D) + lane / (D / 16);
-  if (row >= p.rows) return;
-  const int s = p.starts ? last_not_above(p.num_seqs, row, [&](int i) { return (int64_t)p.starts[i]; }) : (int)row;
-  if (s < 0 || s >= p.num_seqs) return;
+  const int64_t row0 = (int64_t)(item / chunks) * (1024 / D), row = row0 + lane / (D / 16);
+  int s = (int)row;
+  if (p.starts) {   // the first row's sequence, and from there to the lane's own
+    s = last_not_above(p.num_seqs, row0, lane, [&](int i) { return (int64_t)p.starts[i]; });
+    if (s < 0) s = 0;
+    while (s + 1 < p.num_seqs && p.starts[s + 1] <= row) ++s;
+  }
+  if (row >= p.rows || s >= p.num_seqs) return;
   const NewRows rows = new_rows(p, s);
   const int64_t place = rows.base + row;
   if (row < rows.begin || row >= rows.end || place < 0 || place >= position_limit(p)) return;
-  const int64_t blk = block_of_table(p, s, place / p.block_size);
-  if (blk < 0 || blk >= p.num_blocks) return;
-  const RotaryPlace at = rotary_place<D>(lane, p.rotary);
-  Turn tr;
-  if (p.rotary > 0) tr = load_turn<INTER>(p.cos, p.sin, p.table_stride, place, p.table_rows, at);
-  const int64_t to = blk * p.c_blk + place % p.block_size * p.c_tok;
+  const RotaryPlace k_at = rotary_place<D>(lane, p.rotary), v_at = rotary_place<D>(lane, 0);
   const T* k = (const T*)p.side[0].x + row * p.side[0].x_row;
   const T* v = (const T*)p.side[1].x + row * p.side[1].x_row;
+  // the first rows and the angles come while the block is looked up
+  RawRow next_k = load_row<T, D, true>(k + h0 * p.side[0].x_head, k_at), next_v = load_row<T, D, true>(v + h0 * p.side[1].x_head, v_at);
+  Turn tr;
+  if (p.rotary > 0) tr = load_turn<INTER>(p.cos, p.sin, p.table_stride, place, p.table_rows, k_at);
+  const int64_t blk = block_of_table(p, s, place / p.block_size);
+  if (blk < 0 || blk >= p.num_blocks) return;
+  const int64_t to = blk * p.c_blk + place % p.block_size * p.c_tok;
   T *kc = (T*)p.side[0].cache + to, *vc = (T*)p.side[1].cache + to;
   for (int h = h0; h < h1; ++h) {
-    u32x4 lo = *(const u32x4*)(k + h * p.side[0].x_head + at.lo), hi = *(const u32x4*)(k + h * p.side[0].x_head + at.hi);
-    const u32x4 vlo = *(const u32x4*)(v + h * p.side[1].x_head + at.lo), vhi = *(const u32x4*)(v + h * p.side[1].x_head + at.hi);
+    RawRow row_k = next_k;
+    const RawRow row_v = next_v;
+    if (h + 1 < h1) {
+      next_k = load_row<T, D, true>(k + (h + 1) * p.side[0].x_head, k_at);
+      next_v = load_row<T, D, true>(v + (h + 1) * p.side[1].x_head, v_at);
+    }
     if (p.rotary > 0) {
       float x[16];
-      unpack8<T>(lo, x);
-      unpack8<T>(hi, x + 8);
-      turn<INTER, 1>(x, tr, at.turned);
-      lo = pack8<T>(x);
-      hi = pack8<T>(x + 8);
+      unpack_row<T>(row_k, x);
+      turn<INTER, 1>(x, tr, k_at.turned);
+      row_k = RawRow{pack8<T>(x), pack8<T>(x + 8)};
     }
-    *(u32x4*)(kc + h * p.c_head + at.lo) = lo;
-    *(u32x4*)(kc + h * p.c_head + at.hi) = hi;
-    *(u32x4*)(vc + h * p.c_head + at.lo) = vlo;
-    *(u32x4*)(vc + h * p.c_head + at.hi) = vhi;
+    store_raw(kc + h * p.c_head, k_at, row_k);
+    store_raw(vc + h * p.c_head, v_at, row_v);
   }
 }
 
@@ -122,17 +138,16 @@ template <class T, int D, bool INTER>
 FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) append_e4m3_kernel(AppendParams p) {
   constexpr int ROWS = 1024 / D;   // rows that a wavefront holds at a time
   const int lane = hw::thread_id() & 63;
-  // The four wavefronts of a workgroup share a segment: one block of one sequence.
-  const int per_segment = (2 * p.Hkv + kAppendWaves - 1) / kAppendWaves;
+  // The four wavefronts of a workgroup share a segment, one block of one sequence, and have a head each.
+  const int per_segment = (p.Hkv + kAppendWaves - 1) / kAppendWaves;
   const int segment = hw::block_x() / per_segment;
-  const int job = hw::uniform(hw::block_x() % per_segment * kAppendWaves + (hw::thread_id() >> 6));
-  if (job >= 2 * p.Hkv) return;
-  const int h = job >> 1, side = job & 1;
+  const int h = hw::uniform(hw::block_x() % per_segment * kAppendWaves + (hw::thread_id() >> 6));
+  if (h >= p.Hkv) return;
   // Sequence s has the segments from starts[s] / block + 2 s on: at least as many as the blocks its rows can touch.
   int s = segment, nth = 0;
   if (p.starts) {
     auto first = [&](int i) { return clamp64(p.starts[i], 0, p.rows) / p.block_size + 2 * (int64_t)i; };
-    s = hw::uniform(last_not_above(p.num_seqs, segment, first));
+    s = last_not_above(p.num_seqs, segment, lane, first);
     if (s < 0) return;
     nth = (int)(segment - first(s));
   }
@@ -142,71 +157,117 @@ FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) append_e4m3_kernel(AppendParams p) {
   const int64_t column = begin / p.block_size + nth, at0 = column * p.block_size;
   const int64_t from = at0 > begin ? at0 : begin, to = at0 + p.block_size < end ? at0 + p.block_size : end;
   if (from >= to) return;
-  const int64_t blk = block_of_table(p, s, column);
-  if (blk < 0 || blk >= p.num_blocks) return;
+  const int64_t blk = block_of_table(p, s, column);   // comes along with the rows, which do not need it
   const int slot0 = (int)(from - at0), count = (int)(to - from);
-
-  const AppendSide& sd = p.side[side];
-  const bool turns = side == 0 && p.rotary > 0;
-  const RotaryPlace at = rotary_place<D>(lane, turns ? p.rotary : 0);
+  const RotaryPlace turned_at = rotary_place<D>(lane, p.rotary), plain_at = rotary_place<D>(lane, 0);
   const int r0 = lane / (D / 16);
-  const T* x = (const T*)sd.x + (from - rows.base) * sd.x_row + h * sd.x_head;   // row of position `from`
-  uint8_t* cache = (uint8_t*)sd.cache + blk * p.c_blk + h * p.c_head;
-  float* scale = sd.scale + blk * p.s_blk + h * p.s_head;
 
-  auto load = [&](int r, float* v) {
-    unpack8<T>(*(const u32x4*)(x + r * sd.x_row + at.lo), v);
-    unpack8<T>(*(const u32x4*)(x + r * sd.x_row + at.hi), v + 8);
-    if (turns) turn<INTER, 1>(v, load_turn<INTER>(p.cos, p.sin, p.table_stride, from + r, p.table_rows, at), at.turned);
-  };
-  const float before = *scale;   // requested in front of everything that takes time, and of the exchanges that join the lanes
-  float peak = 0.f;
-  for (int r = r0; r < count; r += ROWS) {
-    float v[16];
-    load(r, v);
+  // Keys (side 0) and values.  The first ROWS rows of each stay in registers as they were loaded; what is behind them is
+  // read twice, the second time from the caches (twice as many in registers leave fewer wavefronts: 27.1 and not 26.3 us for
+  // 16384 rows of 8 heads, D = 128, in blocks of 16).
+  RawRow kept[2];
+  Turn kept_turn;
+  float before[2];
+  const T* x[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) peak = fmaxf(peak, finite_magnitude(v[i]));
+  for (int side = 0; side < 2; ++side) {
+    const AppendSide& sd = p.side[side];
+    x[side] = (const T*)sd.x + (from - rows.base) * sd.x_row + h * sd.x_head;   // row of position `from`
+    // (past the last row: the last one again, not counted)
+    kept[side] = load_row<T, D, true>(x[side] + imin(r0, count - 1) * sd.x_row, side ? plain_at : turned_at);
   }
+  if (p.rotary > 0) kept_turn = load_turn<INTER>(p.cos, p.sin, p.table_stride, from + imin(r0, count - 1), p.table_rows, turned_at);
+  if (blk < 0 || blk >= p.num_blocks) return;
 #pragma unroll
-  for (int m = 1; m < 64; m *= 2) peak = fmaxf(peak, hw::shfl_xor(peak, m));
-  float now = scale_for_peak(peak);
-  if (slot0 > 0) {
-    if (now > before) {
-      const float shrink = before / now;
-      for (int r = r0; r < slot0; r += ROWS) {
+  for (int side = 0; side < 2; ++side) before[side] = p.side[side].scale[blk * p.s_blk + h * p.s_head];
+
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    const AppendSide& sd = p.side[side];
+    const RotaryPlace at = side ? plain_at : turned_at;
+    uint8_t* cache = (uint8_t*)sd.cache + blk * p.c_blk + h * p.c_head;
+    // each(row, whether it exists, values): all lanes together, those without a row with the last one.  (The rows that are
+    // kept stand in front of the loop, not in it: 28.3 and not 31.9 us at the size above.)
+    auto for_rows = [&](auto&& each) {
+      float v[16];
+      unpack_row<T>(kept[side], v);
+      if (side == 0 && p.rotary > 0) turn<INTER, 1>(v, kept_turn, at.turned);
+      each(r0, r0 < count, v);
+      for (int first = ROWS; first < count; first += ROWS) {
+        const int r = imin(first + r0, count - 1);
+        Turn t;
+        if (side == 0 && p.rotary > 0) t = load_turn<INTER>(p.cos, p.sin, p.table_stride, from + r, p.table_rows, at);
+        unpack_row<T>(load_row<T, D, false>(x[side] + r * sd.x_row, at), v);
+        if (side == 0 && p.rotary > 0) turn<INTER, 1>(v, t, at.turned);
+        each(r, first + r0 < count, v);
+      }
+    };
+    float peak = 0.f;
+    for_rows([&](int, bool, const float* v) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) peak = fmaxf(peak, finite_magnitude(v[i]));
+    });
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) peak = fmaxf(peak, hw::shfl_xor(peak, m));
+    float now = scale_for_peak(peak);
+    if (slot0 > 0) {
+      if (now > before[side]) {
+        const float shrink = before[side] / now;
+        for (int r = r0; r < slot0; r += ROWS) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            hw::u32x2* codes = (hw::u32x2*)(cache + r * p.c_tok + (i ? at.hi : at.lo));
+            hw::u32x2 c = *codes;
+            c[0] = hw::to_e4m3(hw::from_e4m3(c[0]) * shrink);
+            c[1] = hw::to_e4m3(hw::from_e4m3(c[1]) * shrink);
+            *codes = c;
+          }
+        }
+      } else {
+        now = before[side];
+      }
+    }
+    const float inverse = 1.f / now;
+    for_rows([&](int r, bool there, const float* v) {
+      uint8_t* row = cache + (slot0 + r) * p.c_tok;
+      hw::u32x2 lo = codes8(v, inverse), hi = codes8(v + 8, inverse);
+      if (D >= 32 && (side || p.rotary % 32 == 0)) {
+        // The lanes of a pair have sixteen codes side by side in their first halves, and in their second: one takes those,
+        // the other these, so that a row is one store.
+        const bool odd = lane & 1;
+        const hw::u32x2 give = odd ? lo : hi, keep = odd ? hi : lo;
+        hw::u32x2 got;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          hw::u32x2* codes = (hw::u32x2*)(cache + r * p.c_tok + (i ? at.hi : at.lo));
-          hw::u32x2 c = *codes;
-          c[0] = hw::to_e4m3(hw::from_e4m3(c[0]) * shrink);
-          c[1] = hw::to_e4m3(hw::from_e4m3(c[1]) * shrink);
-          *codes = c;
+          const uint32_t word = give[i];   // (a cast of the vector's element itself reads element 0)
+          got[i] = __builtin_bit_cast(uint32_t, hw::shfl_xor(__builtin_bit_cast(float, word), 1));
         }
+        const u32x4 both = odd ? u32x4{got[0], got[1], keep[0], keep[1]} : u32x4{keep[0], keep[1], got[0], got[1]};
+        if (there) {
+          uint8_t* to_codes = row + (odd ? at.hi - 8 : at.lo);
+          if (D >= 64) hw::store_once(to_codes, both);   // whole lines where a block's rows follow each other
+          else *(u32x4*)to_codes = both;
+        }
+      } else if (there) {
+        *(hw::u32x2*)(row + at.lo) = lo;
+        *(hw::u32x2*)(row + at.hi) = hi;
       }
-    } else {
-      now = before;
-    }
+    });
+    if (lane == 0) sd.scale[blk * p.s_blk + h * p.s_head] = now;
   }
-  const float inverse = 1.f / now;
-  for (int r = r0; r < count; r += ROWS) {
-    float v[16];
-    load(r, v);
-    uint8_t* row = cache + (slot0 + r) * p.c_tok;
-    *(hw::u32x2*)(row + at.lo) = codes8(v, inverse);
-    *(hw::u32x2*)(row + at.hi) = codes8(v + 8, inverse);
-  }
-  if (lane == 0) *scale = now;
 }
 
 template <class T, int D, bool INTER>
 static int launch_append_d(AppendParams p, hipStream_t stream) {
   if (p.side[0].scale) {
-    const int per_segment = (2 * p.Hkv + kAppendWaves - 1) / kAppendWaves;
+    const int per_segment = (p.Hkv + kAppendWaves - 1) / kAppendWaves;
     const unsigned wgs = workgroups({p.starts ? p.rows / p.block_size + 2 * (int64_t)p.num_seqs : p.num_seqs, per_segment});
     return wgs ? launch(append_e4m3_kernel<T, D, INTER>, dim3(wgs), 0, stream, p) : kBadArgument;
   }
-  const int64_t groups = (p.rows + 1024 / D - 1) / (1024 / D), waves = 32 * (int64_t)num_cus_of_current_device();
-  const int64_t n = waves > 0 ? groups * p.Hkv / waves : 1;   // heads per item: as many as leave each SIMD eight wavefronts
+  const int64_t groups = (p.rows + 1024 / D - 1) / (1024 / D), cus = num_cus_of_current_device();
+  // Heads per item: as many as leave each SIMD four wavefronts, eight where rows are narrower than a line (16384 rows of 8
+  // heads, D = 128: 27.6 us with four, 29.3 with eight; 8755 of 32, D = 64: 36.8 and 34.1).
+  const int64_t waves = (D >= 128 ? 16 : 32) * cus, n = waves > 0 ? groups * p.Hkv / waves : 1;
   p.heads_per_item = (int)(n < 1 ? 1 : n > p.Hkv ? p.Hkv : n);
   const int chunks = (p.Hkv + p.heads_per_item - 1) / p.heads_per_item;
   const unsigned wgs = workgroups({(groups * chunks + kAppendWaves - 1) / kAppendWaves});

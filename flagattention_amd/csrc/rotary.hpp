@@ -74,4 +74,18 @@ FA_DEVICE u32x4 pack8(const float* x) {
   return r;
 }
 
+// A lane's share of a row as it lies in memory.  ONCE: marked non-temporal where each of the two loads takes whole 128-byte
+// lines (a line of which another load wants the rest may be gone by then).
+struct RawRow { u32x4 lo, hi; };
+template <class T, int D, bool ONCE>
+FA_DEVICE RawRow load_row(const T* row, RotaryPlace at) {
+  if constexpr (D >= 128 && ONCE) return RawRow{hw::load_once<u32x4>(row + at.lo), hw::load_once<u32x4>(row + at.hi)};
+  else return RawRow{*(const u32x4*)(row + at.lo), *(const u32x4*)(row + at.hi)};
+}
+template <class T>
+FA_DEVICE void unpack_row(const RawRow& r, float* x) {
+  unpack8<T>(r.lo, x);
+  unpack8<T>(r.hi, x + 8);
+}
+
 }  // namespace fa
