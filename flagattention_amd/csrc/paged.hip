@@ -249,7 +249,7 @@ FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) paged_balanced_reduce_kernel(PagedPara
   const int G = p.Hq / p.Hkv;
   const int rows = imin(16, G - rb * 16), n = follow + 1;
   int side = 1;                                    // rows at a time: a power of two of at most kSets
-  while (side < kSets && side < rows) side *= 2;
+  while (side < kSets && side < rows && side != p.merge_rows) side *= 2;
   const int shares = kSets / side;                 // threads that share a row's partials
   const int set = tid / kLanes, share = set / side, d = (tid % kLanes) * 4;
   float* area = (float*)smem;                      // value e of thread t at [e][t]
@@ -329,7 +329,8 @@ FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) paged_balanced_reduce_kernel(PagedPara
 
 template <class T>
 static int launch_balanced_reduce(const PagedParams& p, hipStream_t stream) {
-  const int group = p.Hq / p.Hkv, at_once = 1024 / p.D;   // rows of a pair, and those that a workgroup has threads for
+  const int group = p.Hq / p.Hkv;   // rows of a pair, and those that a workgroup has
+  const int at_once = p.merge_rows > 0 && p.merge_rows < 1024 / p.D ? p.merge_rows : 1024 / p.D;
   dim3 grid(p.num_wgs, ((group < 16 ? group : 16) + at_once - 1) / at_once, 1);
   constexpr size_t lds = 6 * kThreads * sizeof(float);
   switch (p.D) {

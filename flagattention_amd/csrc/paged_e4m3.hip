@@ -28,7 +28,9 @@ namespace fa {
 template <int D>
 struct E4m3Cfg {
   static constexpr int TK = 32;                        // keys per wavefront step: the contraction of one second product
-  static constexpr int WAVES = D <= 64 ? 4 : D == 128 ? 3 : D == 256 ? 2 : 1;   // wavefronts per SIMD that the registers allow
+  // wavefronts per SIMD that the registers allow, in a balanced launch and with a workgroup to a pair (300 sequences of 1 ..
+  // 700 keys, 16 heads, D = 64: 43.5 us with five, 47.2 with four)
+  static constexpr int WAVES = D <= 64 ? 4 : D == 128 ? 3 : D == 256 ? 2 : 1, WAVES_ALONE = D <= 64 ? 5 : WAVES;
   static constexpr int KB_BYTES = D / 4;               // codes of a key that a lane holds for the first product
   static constexpr int KW = KB_BYTES / 4;              // in dwords
   static constexpr int KSTEPS = D < 32 ? 1 : D / 32;   // products over the head size
@@ -437,7 +439,7 @@ FA_DEVICE const T* e4m3_query_row(const PagedParams& p, int seq, int hk, int rb)
 
 // One workgroup per (sequence, kv head, 16 query heads).
 template <class T, int D, bool OCTETS>
-FA_KERNEL void FA_LAUNCH_BOUNDS2(kThreads, E4m3Cfg<D>::WAVES) paged_e4m3_kernel(PagedParams p) {
+FA_KERNEL void FA_LAUNCH_BOUNDS2(kThreads, E4m3Cfg<D>::WAVES_ALONE) paged_e4m3_kernel(PagedParams p) {
   FA_LDS_DECL(smem);
   const int G = p.Hq / p.Hkv, row_blocks = (G + 15) / 16;
   const int rb = hw::block_x() % row_blocks, hk = hw::block_x() / row_blocks % p.Hkv, seq = hw::block_x() / row_blocks / p.Hkv;
@@ -482,7 +484,14 @@ static int launch_e4m3_d(const PagedParams& p, hipStream_t stream) {
   if (p.num_wgs > 0) {
     PagedParams r = p;
     int rc;
-    if ((int64_t)4 * p.num_seqs * p.Hkv * row_blocks <= p.num_wgs) {
+    const int64_t pairs = (int64_t)p.num_seqs * p.Hkv * row_blocks;
+    if (4 * pairs <= p.num_wgs) {
+      // Of the threads that the merge has for the rows of a pair, as many share a row as leave each about sixteen of its
+      // partial results.
+      constexpr int kSets = 1024 / D;
+      int shares = 1;
+      while (shares < kSets && 32 * shares * pairs <= p.num_wgs) shares *= 2;
+      r.merge_rows = kSets / shares;
       rc = launch(paged_e4m3_pieces_kernel<T, D, OCTETS>, dim3(p.num_wgs), lds, stream, p);
     } else {
       rc = launch(paged_e4m3_ranges_kernel<T, D, OCTETS>, dim3(p.num_wgs), 4 * E4m3Cfg<D>::PATCH, stream, p);

@@ -132,6 +132,7 @@ struct PagedParams {
   int dtype;
   // balanced launch only: partial results of workgroups that share a (sequence, kv head) pair
   float* ws; int num_wgs;
+  int merge_rows;   // rows of a pair that a workgroup of the merge has at most (a power of two; 0: as many as there are threads for)
   // caches of e4m3 codes only: scales (num_blocks, Hkv), and the extents that block numbers are held to
   const float *k_scales, *v_scales; int64_t scale_sblk, scale_sh;
   int num_blocks, bt_cols;
