@@ -314,6 +314,38 @@ def test_norm_rotary_refuses():
             pytest.fail(str(list(change)))
 
 
+# ------------------------------------------------------------------------------------- order of the wavefronts ----
+def test_results_do_not_depend_on_how_the_wavefronts_advance(monkeypatch, simulator_behind_the_public_api):
+    """Bit for bit under every order that the barriers allow: a missing one would show."""
+    from flagattention_amd import _abi
+    lib = simulator_behind_the_public_api
+    attends = [cases.attention_inputs(FP16, [150, 0, 290], 4, 2, D, 16, seed=51) for D in (64, 128)]
+    appends = cases.append_inputs(BF16, 8, [3, 20], [25, 4], 2, 64, 16, 64, 52)
+    rotaries = cases.rotary_inputs(BF16, 2, 4, 2, 9, 64, 64, 53, weight_type=torch.float32, grad=True)
+
+    def everything():
+        got = []
+        for q, *rest, longest in attends:
+            for wgs in (0, 3, 20):     # one workgroup per pair, ranges of wavefronts, pieces of workgroups
+                out = torch.full_like(q, torch.nan)
+                ws = torch.empty(lib.paged_attn_e4m3_workspace(max(1, wgs), q.shape[2]) // 4) if wgs else None
+                _abi.paged_attn_e4m3(lib, out, q, *rest, ws, wgs)
+                got.append(out)
+        a = cases.copied(appends)
+        flag_attn.paged_append(**a)
+        got += [a[n].view(torch.uint8) for n in ("key_cache", "value_cache", "key_scales", "value_scales")]
+        outs = flag_attn.norm_rotary(**rotaries)
+        got += outs
+        got += torch.autograd.grad(outs, [rotaries[n] for n in ("q", "k", "q_weight", "k_weight")], [torch.ones_like(o) for o in outs])
+        return got
+
+    want = everything()
+    for schedule, seed in (("ahead", "0"), ("ahead_descending", "0"), ("random", "1"), ("random", "2")):
+        monkeypatch.setenv("HWSIM_SCHEDULE", schedule)
+        monkeypatch.setenv("HWSIM_SEED", seed)
+        assert all(torch.equal(a, b) for a, b in zip(want, everything())), (schedule, seed)
+
+
 # ------------------------------------------------------------------------------------------------- together ----
 def test_a_prompt_and_steps_behind_it():
     """Norm and rotation of the queries, rotation of the keys on their way into the cache, attention: into 8 and 16 bits."""
