@@ -13,8 +13,8 @@
 // numbers that fall below e4m3's normal range, and costs no precision: the codes are floating-point numbers.
 //
 // Bound by memory (each new value is read and stored once) or, for single tokens, by the chain length -> table -> scale ->
-// store.  A wavefront of the 16-bit kernel holds 1024 / D rows and walks a run of heads; one of the 8-bit kernel has one
-// block of one head, keys and values, so that the scales are its own.
+// store.  A wavefront of the 16-bit kernel holds 1024 / D rows and walks a run of heads; a wavefront or a workgroup of
+// the 8-bit kernel has one block of one head, so that the scales are its own.
 #include "rotary.hpp"
 
 namespace fa {
@@ -134,21 +134,24 @@ FA_DEVICE hw::u32x2 codes8(const float* x, float inverse) {
   return r;
 }
 
-template <class T, int D, bool INTER>
+// SHARED: a workgroup has one block of one head, two wavefronts the keys and two the values, 1024 / D rows in turn.
+// Otherwise a wavefront has one block of one head, keys and values one after the other, and a workgroup four heads.
+template <class T, int D, bool INTER, bool SHARED>
 FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) append_e4m3_kernel(AppendParams p) {
-  constexpr int ROWS = 1024 / D;   // rows that a wavefront holds at a time
-  const int lane = hw::thread_id() & 63;
-  // The four wavefronts of a workgroup share a segment, one block of one sequence, and have a head each.
-  const int per_segment = (p.Hkv + kAppendWaves - 1) / kAppendWaves;
-  const int segment = hw::block_x() / per_segment;
-  const int h = hw::uniform(hw::block_x() % per_segment * kAppendWaves + (hw::thread_id() >> 6));
+  FA_LDS_DECL(smem);
+  constexpr int ROWS = 1024 / D, TURN = SHARED ? 2 * ROWS : ROWS, SIDES = SHARED ? 1 : 2;   // rows held at a time; sides
+  const int lane = hw::thread_id() & 63, wave = hw::uniform(hw::thread_id() >> 6);
+  const int per_segment = SHARED ? p.Hkv : (p.Hkv + kAppendWaves - 1) / kAppendWaves;
+  const int segment = hw::block_x() / per_segment;   // one block of one sequence
+  const int h = hw::block_x() % per_segment * (SHARED ? 1 : kAppendWaves) + (SHARED ? 0 : wave);
   if (h >= p.Hkv) return;
+  const int side0 = SHARED ? wave & 1 : 0, r0 = (SHARED ? wave >> 1 : 0) * ROWS + lane / (D / 16);
   // Sequence s has the segments from starts[s] / block + 2 s on: at least as many as the blocks its rows can touch.
   int s = segment, nth = 0;
   if (p.starts) {
     auto first = [&](int i) { return clamp64(p.starts[i], 0, p.rows) / p.block_size + 2 * (int64_t)i; };
     s = last_not_above(p.num_seqs, segment, lane, first);
-    if (s < 0) return;
+    if (s < 0) return;   // (this return and the next ones: all that share a block of a head together)
     nth = (int)(segment - first(s));
   }
   const NewRows rows = new_rows(p, s);
@@ -159,64 +162,74 @@ FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) append_e4m3_kernel(AppendParams p) {
   if (from >= to) return;
   const int64_t blk = block_of_table(p, s, column);   // comes along with the rows, which do not need it
   const int slot0 = (int)(from - at0), count = (int)(to - from);
-  const RotaryPlace turned_at = rotary_place<D>(lane, p.rotary), plain_at = rotary_place<D>(lane, 0);
-  const int r0 = lane / (D / 16);
 
-  // Keys (side 0) and values.  The first ROWS rows of each stay in registers as they were loaded; what is behind them is
+  // Keys (side 0) and values.  The first TURN rows of each stay in registers as they were loaded; what is behind them is
   // read twice, the second time from the caches (twice as many in registers leave fewer wavefronts: 27.1 and not 26.3 us for
   // 16384 rows of 8 heads, D = 128, in blocks of 16).
-  RawRow kept[2];
+  const RotaryPlace turned_at = rotary_place<D>(lane, p.rotary), plain_at = rotary_place<D>(lane, 0);
+  RawRow kept[SIDES];
   Turn kept_turn;
-  float before[2];
-  const T* x[2];
+  float before[SIDES];
+  const T* x[SIDES];
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const AppendSide& sd = p.side[side];
-    x[side] = (const T*)sd.x + (from - rows.base) * sd.x_row + h * sd.x_head;   // row of position `from`
+  for (int i = 0; i < SIDES; ++i) {
+    const AppendSide& sd = p.side[side0 + i];
+    x[i] = (const T*)sd.x + (from - rows.base) * sd.x_row + h * sd.x_head;   // row of position `from`
     // (past the last row: the last one again, not counted)
-    kept[side] = load_row<T, D, true>(x[side] + imin(r0, count - 1) * sd.x_row, side ? plain_at : turned_at);
+    kept[i] = load_row<T, D, true>(x[i] + imin(r0, count - 1) * sd.x_row, side0 + i ? plain_at : turned_at);
   }
-  if (p.rotary > 0) kept_turn = load_turn<INTER>(p.cos, p.sin, p.table_stride, from + imin(r0, count - 1), p.table_rows, turned_at);
+  if (p.rotary > 0 && side0 == 0)
+    kept_turn = load_turn<INTER>(p.cos, p.sin, p.table_stride, from + imin(r0, count - 1), p.table_rows, turned_at);
   if (blk < 0 || blk >= p.num_blocks) return;
 #pragma unroll
-  for (int side = 0; side < 2; ++side) before[side] = p.side[side].scale[blk * p.s_blk + h * p.s_head];
+  for (int i = 0; i < SIDES; ++i) before[i] = p.side[side0 + i].scale[blk * p.s_blk + h * p.s_head];
 
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
+  for (int i = 0; i < SIDES; ++i) {
+    const int side = side0 + i;
     const AppendSide& sd = p.side[side];
+    const bool turns = side == 0 && p.rotary > 0;
     const RotaryPlace at = side ? plain_at : turned_at;
     uint8_t* cache = (uint8_t*)sd.cache + blk * p.c_blk + h * p.c_head;
     // each(row, whether it exists, values): all lanes together, those without a row with the last one.  (The rows that are
     // kept stand in front of the loop, not in it: 28.3 and not 31.9 us at the size above.)
     auto for_rows = [&](auto&& each) {
       float v[16];
-      unpack_row<T>(kept[side], v);
-      if (side == 0 && p.rotary > 0) turn<INTER, 1>(v, kept_turn, at.turned);
+      unpack_row<T>(kept[i], v);
+      if (turns) turn<INTER, 1>(v, kept_turn, at.turned);
       each(r0, r0 < count, v);
-      for (int first = ROWS; first < count; first += ROWS) {
+      for (int first = TURN; first < count; first += TURN) {
         const int r = imin(first + r0, count - 1);
         Turn t;
-        if (side == 0 && p.rotary > 0) t = load_turn<INTER>(p.cos, p.sin, p.table_stride, from + r, p.table_rows, at);
-        unpack_row<T>(load_row<T, D, false>(x[side] + r * sd.x_row, at), v);
-        if (side == 0 && p.rotary > 0) turn<INTER, 1>(v, t, at.turned);
+        if (turns) t = load_turn<INTER>(p.cos, p.sin, p.table_stride, from + r, p.table_rows, at);
+        unpack_row<T>(load_row<T, D, false>(x[i] + r * sd.x_row, at), v);
+        if (turns) turn<INTER, 1>(v, t, at.turned);
         each(r, first + r0 < count, v);
       }
     };
     float peak = 0.f;
     for_rows([&](int, bool, const float* v) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) peak = fmaxf(peak, finite_magnitude(v[i]));
+      for (int j = 0; j < 16; ++j) peak = fmaxf(peak, finite_magnitude(v[j]));
     });
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) peak = fmaxf(peak, hw::shfl_xor(peak, m));
+    if (SHARED) {
+      // Also where the other wavefront has no rows: its rows below are those that change to the new scale, and the scale
+      // is not written before all have read the old one.
+      float* peaks = (float*)smem;
+      if (lane == 0) peaks[wave] = peak;
+      hw::block_sync();
+      peak = fmaxf(peaks[side], peaks[side + 2]);
+    }
     float now = scale_for_peak(peak);
     if (slot0 > 0) {
-      if (now > before[side]) {
-        const float shrink = before[side] / now;
-        for (int r = r0; r < slot0; r += ROWS) {
+      if (now > before[i]) {
+        const float shrink = before[i] / now;
+        for (int r = r0; r < slot0; r += TURN) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            hw::u32x2* codes = (hw::u32x2*)(cache + r * p.c_tok + (i ? at.hi : at.lo));
+          for (int j = 0; j < 2; ++j) {
+            hw::u32x2* codes = (hw::u32x2*)(cache + r * p.c_tok + (j ? at.hi : at.lo));
             hw::u32x2 c = *codes;
             c[0] = hw::to_e4m3(hw::from_e4m3(c[0]) * shrink);
             c[1] = hw::to_e4m3(hw::from_e4m3(c[1]) * shrink);
@@ -224,23 +237,23 @@ FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) append_e4m3_kernel(AppendParams p) {
           }
         }
       } else {
-        now = before[side];
+        now = before[i];
       }
     }
     const float inverse = 1.f / now;
     for_rows([&](int r, bool there, const float* v) {
       uint8_t* row = cache + (slot0 + r) * p.c_tok;
       hw::u32x2 lo = codes8(v, inverse), hi = codes8(v + 8, inverse);
-      if (D >= 32 && (side || p.rotary % 32 == 0)) {
+      if (D >= 32 && (!turns || p.rotary % 32 == 0)) {
         // The lanes of a pair have sixteen codes side by side in their first halves, and in their second: one takes those,
         // the other these, so that a row is one store.
         const bool odd = lane & 1;
         const hw::u32x2 give = odd ? lo : hi, keep = odd ? hi : lo;
         hw::u32x2 got;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t word = give[i];   // (a cast of the vector's element itself reads element 0)
-          got[i] = __builtin_bit_cast(uint32_t, hw::shfl_xor(__builtin_bit_cast(float, word), 1));
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t word = give[j];   // (a cast of the vector's element itself reads element 0)
+          got[j] = __builtin_bit_cast(uint32_t, hw::shfl_xor(__builtin_bit_cast(float, word), 1));
         }
         const u32x4 both = odd ? u32x4{got[0], got[1], keep[0], keep[1]} : u32x4{keep[0], keep[1], got[0], got[1]};
         if (there) {
@@ -253,16 +266,26 @@ FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) append_e4m3_kernel(AppendParams p) {
         *(hw::u32x2*)(row + at.hi) = hi;
       }
     });
-    if (lane == 0) sd.scale[blk * p.s_blk + h * p.s_head] = now;
+    if (lane == 0 && wave < (SHARED ? 2 : kAppendWaves)) sd.scale[blk * p.s_blk + h * p.s_head] = now;
   }
 }
 
 template <class T, int D, bool INTER>
 static int launch_append_d(AppendParams p, hipStream_t stream) {
   if (p.side[0].scale) {
-    const int per_segment = (p.Hkv + kAppendWaves - 1) / kAppendWaves;
-    const unsigned wgs = workgroups({p.starts ? p.rows / p.block_size + 2 * (int64_t)p.num_seqs : p.num_seqs, per_segment});
-    return wgs ? launch(append_e4m3_kernel<T, D, INTER>, dim3(wgs), 0, stream, p) : kBadArgument;
+    const int64_t segments = p.starts ? p.rows / p.block_size + 2 * (int64_t)p.num_seqs : p.num_seqs;
+    // A wavefront walks the rows of its block 1024 / D at a time, and twice: a long chain where a block has many, and exposed
+    // where few blocks have rows.  Four are worth their exchange of peaks and their empty places then (alone / shared, us:
+    // 16384 rows of 8 heads, D = 128, blocks of 64: 35.4 / 30.5, of 32: 27.4 / 31.9, of 16: 29.5 / 37.2; 40 rows for each
+    // of 205 sequences in blocks of 64: 18.4 / 21.6; D = 256, blocks of 128: 89.5 / 38.4; 960 rows, D = 128, blocks of 16,
+    // 736 wavefronts alone: 8.3 / 6.4, twice as many rows 9.7 / 9.2, four times 12.1 / 14.0).
+    const int64_t rows = (p.rows + p.num_seqs - 1) / p.num_seqs, per_block = rows < p.block_size ? rows : p.block_size;
+    if (per_block >= 8 * (1024 / D) || segments * p.Hkv <= 4 * (int64_t)num_cus_of_current_device()) {
+      const unsigned wgs = workgroups({segments, p.Hkv});
+      return wgs ? launch(append_e4m3_kernel<T, D, INTER, true>, dim3(wgs), kAppendWaves * sizeof(float), stream, p) : kBadArgument;
+    }
+    const unsigned wgs = workgroups({segments, (p.Hkv + kAppendWaves - 1) / kAppendWaves});
+    return wgs ? launch(append_e4m3_kernel<T, D, INTER, false>, dim3(wgs), 0, stream, p) : kBadArgument;
   }
   const int64_t groups = (p.rows + 1024 / D - 1) / (1024 / D), cus = num_cus_of_current_device();
   // Heads per item: as many as leave each SIMD four wavefronts, eight where rows are narrower than a line (16384 rows of 8

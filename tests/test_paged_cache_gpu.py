@@ -90,6 +90,19 @@ def test_append_to_many_sequences(bits):
     cases.check_append(cases.append_inputs(BF16, bits, olds, news, 2, 64, 16, 64, 22, device="cuda", pad=9))
 
 
+@pytest.mark.parametrize("rotary", [0, 32, 48, 128])
+@pytest.mark.parametrize("olds,news,block", [
+    ([(7 * i) % 40 for i in range(80)], [(11 * i) % 60 for i in range(80)], 16),     # a wavefront for a block of a head
+    ([(7 * i) % 70 for i in range(40)], [70 + (11 * i) % 60 for i in range(40)], 64),   # a workgroup, also of part of a block
+    ([5, 63, 64, 0], [1, 2, 9, 17], 64),                                             # a workgroup, also with rows for one wavefront
+])
+def test_append_to_8_bits_by_wavefronts_and_by_workgroups(olds, news, block, rotary):
+    """Blocks that hold tokens already, with larger and with smaller scales than the new ones need."""
+    args = cases.append_inputs(BF16, 8, olds, news, 8, 128, block, rotary, 34, device="cuda", pad=7)
+    args["key_scales"][::2] = args["value_scales"][::2] = 2.0 ** -9
+    cases.check_append(args)
+
+
 @pytest.mark.parametrize("values", [1e-3, 40.0, 3e4])
 def test_append_makes_room_for_larger_values(values):
     args = cases.append_inputs(FP16 if values < 1e4 else BF16, 8, [9, 3, 0], [1, 4, 30], 2, 64, 16, 64, 23, device="cuda", values=values)

@@ -150,6 +150,14 @@ def test_append(bits, dtype, olds, news, Hkv, D, block, size, interleaved, pad):
     cases.check_append(args)
 
 
+def test_append_by_wavefronts():
+    """So many blocks that each of a head has one wavefront; blocks that hold tokens, and rows that fill two of them."""
+    olds, news = [(7 * i) % 9 for i in range(120)], [1 + (5 * i) % 5 * (i % 8 == 0) * 4 for i in range(120)]
+    args = cases.append_inputs(BF16, 8, olds, news, 5, 128, 12, 128, 28, pad=3)
+    args["key_scales"][::2] = args["value_scales"][::2] = 2.0 ** -9
+    cases.check_append(args)
+
+
 def test_append_makes_room_for_larger_values():
     """Values far above what the block holds: the scale grows, what is there is rounded again, to zero where it falls short."""
     for values in (1e-3, 40.0, 3e4):
