@@ -36,7 +36,8 @@ def append(key, value, key_cache, value_cache, context_lens, block_tables, query
     the cache needs it right after: the last row of s goes to position ``context_lens[s] - 1``.  Rows that have no place are
     not stored: rows behind the last sequence's, of negative position (a padding sequence of length 0), behind the block
     table or the rotation's tables, or whose entry in ``block_tables`` (num_seqs, max_blocks_per_seq) is not a block of the
-    cache.  The blocks that a call stores to belong to one sequence each.
+    cache.  The blocks that a call stores to belong to one sequence each, and stand in
+    its row of the table once.
 
     ``cos``, ``sin`` (positions, rotary size / 2), float32: the first ``rotary size`` values of every key are turned by row
     ``position`` of the tables, in pairs (i, i + size / 2) or, ``interleaved``, (2i, 2i + 1).

@@ -912,6 +912,7 @@ struct RotaryNode : torch::autograd::Function<RotaryNode> {
     const auto qs = ctx->saved_data["q"].toIntVector(), kshape = ctx->saved_data["k"].toIntVector();
     const Tensor& some = grads[0].defined() ? grads[0] : grads[1];
     if (!some.defined()) return variable_list(6);
+    TORCH_CHECK(!at::GradMode::is_enabled(), "norm_rotary is differentiable once: its gradients cannot be part of a graph (create_graph)");
     const c10::DeviceGuard guard(some.device());
     // the gradient of an output that nothing flows into is zero
     const Tensor gq = grads[0].defined() ? kernel_ready(grads[0]) : at::zeros(qs, some.options()),

@@ -30,6 +30,11 @@ constexpr int kMinUnitsPerWg = 2;   // where a range may cross pairs
 
 FA_DEVICE int balanced_slot_floats(int D) { return 16 * D + 32; }
 
+FA_DEVICE int bounded_length(const PagedParams& p, int seq) {
+  const int n = imax(0, p.context_lens[seq]);
+  return p.max_keys > 0 ? imin(n, p.max_keys) : n;
+}
+
 // Runs pair(seq, hk, rb, n_begin, n_end, whole, slot index) for every piece of a pair in this workgroup's range, and clears
 // the output rows of empty sequences.  STEP_KEYS: the keys of a wavefront's step.  WAVES: every wavefront has a range of its
 // own, in units of one step (the workgroups above are wavefronts then, four times as many), and pieces are dealt so however
@@ -46,7 +51,7 @@ FA_DEVICE void balanced_walk(const PagedParams& p, const int D, Pair pair) {
   const int pairs_per_seq = p.Hkv * row_blocks;
 
   // ---- every wavefront scans the context lengths for itself, 64 at a time: no LDS, no barrier ----
-  auto length_of = [&](int s) { return s < p.num_seqs ? imax(0, p.context_lens[s]) : 0; };
+  auto length_of = [&](int s) { return s < p.num_seqs ? bounded_length(p, s) : 0; };
   const int first_lengths = length_of(lane);   // both scans begin with these
   const int64_t num_pairs = (int64_t)p.num_seqs * pairs_per_seq;
   const bool one_each = !WAVES && 4 * num_pairs <= num_wgs;
@@ -110,7 +115,7 @@ FA_DEVICE void balanced_walk(const PagedParams& p, const int D, Pair pair) {
   int unfinished = 0;
 
   while (u < u_end) {
-    const int ctx = hw::uniform(p.context_lens[seq]);
+    const int ctx = hw::uniform(bounded_length(p, seq));
     const int us = ctx > 0 ? cdiv(ctx, unit_keys) : 0;
     const int local = (int)(u - (int64_t)before * pairs_per_seq);  // unit index inside this sequence's pairs
     if (us == 0 || local >= us * pairs_per_seq) { before += us; ++seq; continue; }

@@ -445,7 +445,7 @@ FA_KERNEL void FA_LAUNCH_BOUNDS2(kThreads, E4m3Cfg<D>::WAVES_ALONE) paged_e4m3_k
   const int rb = hw::block_x() % row_blocks, hk = hw::block_x() / row_blocks % p.Hkv, seq = hw::block_x() / row_blocks / p.Hkv;
   E4m3Result<D> res;
   DecodeOut<D> out;
-  decode_e4m3<T, D, OCTETS, 4>(e4m3_source(p, seq, hk), e4m3_query_row<T>(p, seq, hk, rb), 0, imax(0, p.context_lens[seq]),
+  decode_e4m3<T, D, OCTETS, 4>(e4m3_source(p, seq, hk), e4m3_query_row<T>(p, seq, hk, rb), 0, bounded_length(p, seq),
                                p.scale * kLog2e, smem, res);
   join_wavefronts<D>(res, imin(16, G - rb * 16), smem, out);
   store_balanced<T, D>(p, out, kLn2, seq, hk, rb, true, 0);
@@ -516,9 +516,13 @@ static int launch_e4m3(const PagedParams& p, hipStream_t stream) {
   return kUnsupported;
 }
 
-int run_paged_e4m3(const PagedParams& p, hipStream_t stream) {
+int run_paged_e4m3(PagedParams p, hipStream_t stream) {
   if (p.num_seqs <= 0 || p.Hq <= 0 || p.Hkv <= 0 || p.Hq % p.Hkv || p.block_size <= 0 || p.bt_cols <= 0 || p.num_blocks <= 0) return kBadArgument;
   if (p.num_wgs < 0 || (p.num_wgs > 0 && !p.ws)) return kBadArgument;
+  // One key behind the table says as much as all of them: a length that is not one ends soon (and the steps' arithmetic, which
+  // goes up to 255 keys past the end, stays below 2^31).
+  const int64_t keys = (int64_t)p.bt_cols * p.block_size + 1;
+  p.max_keys = (int)(keys < 0x7fffffff - 255 ? keys : 0x7fffffff - 255);
   const bool octets = e4m3_octets(p);
   if (p.dtype == kDtypeF16) return octets ? launch_e4m3<hw::half_t, true>(p, stream) : launch_e4m3<hw::half_t, false>(p, stream);
   if (p.dtype == kDtypeBF16) return octets ? launch_e4m3<hw::bf16_t, true>(p, stream) : launch_e4m3<hw::bf16_t, false>(p, stream);

@@ -136,8 +136,9 @@ struct PagedParams {
   // caches of e4m3 codes only: scales (num_blocks, Hkv), and the extents that block numbers are held to
   const float *k_scales, *v_scales; int64_t scale_sblk, scale_sh;
   int num_blocks, bt_cols;
+  int max_keys;     // context lengths count up to here (0: without a bound); filled in at the launch
 };
-int run_paged_e4m3(const PagedParams& p, hipStream_t stream);
+int run_paged_e4m3(PagedParams p, hipStream_t stream);
 
 // Norm and rotation of queries (side 0) and keys (side 1), views of (B, heads, T, D).
 struct RotarySide {

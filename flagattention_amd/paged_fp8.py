@@ -77,7 +77,7 @@ def attention(query, key_cache, value_cache, key_scales, value_scales, context_l
 
     Returns out shaped like ``query``; a sequence of context length 0 gets a zero row, and so does every one where the
     cache or the table is empty.  A key whose block number is not one of the cache's, or whose column is not in the table,
-    makes the rows that see it NaN; nothing is read for it.  Not differentiable."""
+    makes the rows that see it NaN; nothing is read for it (and a length past the table's end takes no longer than one key past it).  Not differentiable."""
     if query.is_cuda:   # native host path (``csrc/host.cpp``); what it does not take is served below
         out = _lib.native().paged_fp8(query, key_cache, value_cache, key_scales, value_scales, context_lens, block_tables,
                                       attn_scale, max_context_len)

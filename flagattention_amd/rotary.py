@@ -35,6 +35,8 @@ class NormRotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq_out, dk_out):
+        if torch.is_grad_enabled():
+            raise RuntimeError("norm_rotary is differentiable once: its gradients cannot be part of a graph (create_graph)")
         q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
         lib = _lib.get()
         dq_out, dk_out = _abi.kernel_ready(dq_out), _abi.kernel_ready(dk_out)
@@ -64,7 +66,8 @@ def norm_rotary(q, k, cos, sin, positions=None, q_weight=None, k_weight=None, ep
     (num_tokens,) for single tokens; without it the position is the token's index.  A position without a row in the tables
     turns by NaN.  All arithmetic is in fp32, rounded once.
 
-    Returns (q_out, k_out), shaped like the inputs.  Differentiable in q, k and the weights; cos and sin get no gradient."""
+    Returns (q_out, k_out), shaped like the inputs.  Differentiable in q, k and the weights, once (not with
+    ``create_graph``); cos and sin get no gradient."""
     if q.is_cuda:   # native host path (``csrc/host.cpp``); what it does not take is served below
         out = _lib.native().norm_rotary(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved)
         if out is not NotImplemented:

@@ -43,6 +43,21 @@ def test_attention_of_many_short_sequences():
     cases.check_attention(args, flag_attn.paged_attention_fp8(*args))
 
 
+def test_lengths_far_past_the_table_end_soon():
+    for longest, lens in ((100, [50, 30, 70]), (9000, [50, 30, 9000])):
+        args = list(cases.attention_inputs(BF16, lens, 4, 2, 64, 16, seed=19, device="cuda"))
+        args[5][0], args[5][2] = 2 ** 31 - 1, 2 ** 31 - 40
+        out = flag_attn.paged_attention_fp8(*args[:-1], longest)
+        assert out[0].isnan().all() and out[2].isnan().all() and out[1].isfinite().all(), longest
+
+
+def test_norm_rotary_is_differentiable_once():
+    args = cases.rotary_inputs(BF16, 1, 2, 2, 6, 64, 64, 37, device="cuda", grad=True)
+    q, k = flag_attn.norm_rotary(**args)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(q.sum() + k.sum(), args["q"], create_graph=True)
+
+
 def test_offsets_past_32_bits():
     """Caches of 5 GiB each, the blocks in use at both ends."""
     blocks, Hkv, block, D = 20480, 8, 256, 128

@@ -80,6 +80,20 @@ def test_attention_reads_nothing_for_entries_outside_the_cache(block):
     cases.check_attention(args, out)
 
 
+@pytest.mark.parametrize("block", [16, 12])
+def test_lengths_far_past_the_table_end_soon(simulator_behind_the_public_api, block):
+    from flagattention_amd import _abi
+    lib = simulator_behind_the_public_api
+    args = list(cases.attention_inputs(BF16, [50, 30, 70], 4, 2, 64, block, seed=19))
+    args[5][0], args[5][2] = 2 ** 31 - 1, 2 ** 31 - 40
+    q, *rest, longest = args
+    for wgs in (0, 3, 40):   # a workgroup per pair, a range per wavefront, a piece per workgroup
+        out = torch.zeros_like(q)
+        ws = torch.empty(lib.paged_attn_e4m3_workspace(max(1, wgs), 64) // 4) if wgs else None
+        _abi.paged_attn_e4m3(lib, out, q, *rest, ws, wgs)
+        assert out[0].isnan().all() and out[2].isnan().all() and out[1].isfinite().all(), wgs
+
+
 def test_nan_and_infinities_that_a_row_sees_make_it_nan():
     args = list(cases.attention_inputs(BF16, [40, 40, 40, 40], 4, 2, 64, 16, seed=15))
     args[0][0, 1, 3] = torch.nan
@@ -288,6 +302,13 @@ def test_gradients_of_part_of_the_outputs_and_inputs():
     assert torch.equal(a, b)
     (ga,), (gb,) = (torch.autograd.grad(t, one, torch.ones_like(t)) for t in (a, b))
     assert torch.equal(ga, gb) and ga.shape == one.shape
+
+
+def test_norm_rotary_is_differentiable_once():
+    args = cases.rotary_inputs(BF16, 1, 2, 2, 6, 64, 64, 37, grad=True)
+    q, k = flag_attn.norm_rotary(**args)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(q.sum() + k.sum(), args["q"], create_graph=True)
 
 
 def test_norm_rotary_of_rows_of_zeros_and_of_nothing():
