@@ -185,9 +185,11 @@ int balanced_workgroups(int64_t seqs, int64_t Hkv, int64_t group, int64_t D, int
 // paged_fp8.choose_workgroups (the reasons and figures stand there)
 int e4m3_workgroups(int64_t seqs, int64_t Hkv, int64_t group, int64_t D, int64_t max_context, int cus) {
   const double pairs = (double)(seqs * Hkv * cdiv(group, 16)), stream = pairs * (double)max_context * (double)D / 5.5e6;
-  const double step = D <= 64 ? 1.05 : D == 128 ? 1.4 : D == 256 ? 2.2 : 4.5, balanced = D <= 128 ? 9.5 : D == 256 ? 12.0 : 15.0;
+  const int wgs = cus * (D <= 64 ? 4 : D <= 256 ? 2 : 1);
+  const double step = D <= 64 ? 1.05 : D == 128 ? 1.4 : D == 256 ? 2.2 : 4.5;
+  const double balanced = 8 * pairs <= wgs ? (D <= 128 ? 9.5 : D == 256 ? 12.0 : 15.0) : D <= 64 ? 12.0 : D == 128 ? 13.0 : D == 256 ? 20.0 : 15.0;
   const double alone = 3.0 + step * (double)cdiv(max_context, 128) + 0.6 * stream;
-  return alone <= balanced + stream ? 0 : cus * (D <= 64 ? 4 : D <= 256 ? 2 : 1);
+  return alone <= balanced + stream ? 0 : wgs;
 }
 
 // ------------------------------------------------------------------------------------------------ tensors ----

@@ -12,9 +12,11 @@ __all__ = ["attention"]
 
 
 # By head size: microseconds that a workgroup alone on its pair takes for 128 keys (four wavefronts, a step each), and that a
-# balanced launch takes before it streams (two kernels, the scan of the context lengths, the merge).
+# balanced launch takes before it streams (two kernels, the scan of the context lengths, the merge), with few pairs (an eighth of
+# its workgroups) and with more, each of which costs partial results.
 _STEP_US = {16: 1.05, 32: 1.05, 64: 1.05, 128: 1.4, 256: 2.2, 512: 4.5}
-_BALANCED_US = {16: 9.5, 32: 9.5, 64: 9.5, 128: 9.5, 256: 12.0, 512: 15.0}
+_FEW_US = {16: 9.5, 32: 9.5, 64: 9.5, 128: 9.5, 256: 12.0, 512: 15.0}
+_BALANCED_US = {16: 12.0, 32: 12.0, 64: 12.0, 128: 13.0, 256: 20.0, 512: 15.0}
 
 
 def choose_workgroups(num_seqs, num_kv_heads, group, head_size, max_context_len, num_cus):
@@ -22,15 +24,18 @@ def choose_workgroups(num_seqs, num_kv_heads, group, head_size, max_context_len,
     that the hardware deals out by itself.  That is as long as the longest sequence takes one workgroup and, with many pairs,
     as the keys' bytes take at 5.5 TB/s, of which the part behind the longest one counts.  Lengths are taken to be spread up
     to the longest.  Measured, one per pair against balanced (us, lengths uniform up to the longest, D = 128):
-    8 pairs of up to 512 keys 8.6 / 9.8, of 1024 13.4 / 10.3; 512 pairs of 1024 22 / 28, of 2048 39.5 / 39.6, of 4096 74 / 66;
-    2048 pairs of 2048 104 / 117; D = 64: 4096 pairs of 1024 61 / 74; D = 256: 4 pairs of 256 9.4 / 12.0, of 512 14 / 12.
+    8 pairs of up to 512 keys 8.6 / 9.8, of 1024 13.4 / 10.3; 256 pairs of 1024 17.4 / 19.1, of 2048 31 / 24; 512 pairs of
+    1024 21 / 27, of 2048 35.5 / 37.1, of 4096 67 / 64, of 8192 133 / 100; 2048 pairs of 2048 104 / 117; D = 64: 256 pairs of
+    1024 14.1 / 13.8, 512 16.3 / 17.7, 4096 61 / 74; D = 32: 256 pairs of 1024 11.3 / 13.1, of 2048 21 / 15; D = 256: 4 pairs
+    of 256 9.4 / 12.0, of 512 14 / 12, 512 pairs of 1024 31 / 35, of 2048 54 / 62, 256 pairs of 2048 39 / 36; D = 512: 96 pairs
+    of 512 23 / 23, of 1024 56 / 28.
     A compute unit holds four workgroups up to head size 64, two up to 256 and one above."""
     pairs = num_seqs * num_kv_heads * (-(-group // 16))
     stream = pairs * max_context_len * head_size / 5.5e6
+    wgs = num_cus * (4 if head_size <= 64 else 2 if head_size <= 256 else 1)
+    fixed = (_FEW_US if 8 * pairs <= wgs else _BALANCED_US)[head_size]
     alone = 3.0 + _STEP_US[head_size] * (-(-max_context_len // 128)) + 0.6 * stream
-    if alone <= _BALANCED_US[head_size] + stream:
-        return 0
-    return num_cus * (4 if head_size <= 64 else 2 if head_size <= 256 else 1)
+    return 0 if alone <= fixed + stream else wgs
 
 
 def check_cache(key_cache, value_cache, key_scales, value_scales):
