@@ -131,6 +131,7 @@ FA_DEVICE uint64_t ballot(bool pred) { return __builtin_amdgcn_ballot_w64(pred);
 // Value held by lane l - delta (lanes below delta keep their own), and by a given lane.
 FA_DEVICE int shfl_up(int x, int delta) { return __shfl_up(x, delta, 64); }
 FA_DEVICE int lane_value(int x, int lane) { return __shfl(x, lane, 64); }
+FA_DEVICE float lane_value(float x, int lane) { return __shfl(x, lane, 64); }
 // Inclusive prefix sum over the 64 lanes: data-parallel-primitive adds inside the rows of 16 lanes, then each row's
 // total into the rows behind it -- six vector instructions, where exchanges through LDS cost a latency each.
 FA_DEVICE int wave_prefix_sum(int x) {

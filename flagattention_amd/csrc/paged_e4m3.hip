@@ -2,11 +2,18 @@
 //   o = sum_n p_n vs_b(n) v_n / sum_n p_n,   p_n = exp(scale ks_b(n) q.k_n),   b(n) the cache block of key n.
 //
 // Bound by memory: a key costs 2 D bytes per kv head, half of what a 16-bit cache costs, so half of the time is left for
-// everything else.  What carries it:
-//   * No LDS on the way.  e4m3 becomes bf16 or fp16 exactly, two numbers per instruction, so the codes are converted in
-//     registers between the load and the matrix product; and the loads put every code where the product wants it, because
-//     the order of the contraction index of a product, and of its rows, is free as long as both operands (and the reader of
-//     the result) agree on it.
+// everything else.  64 sequences of 512 .. 8192 keys, 32 / 8 heads of 128: 97 us for 573 MB, 5.9 TB/s, where loads that do
+// nothing else reach 6.5 (and the merge behind it 5); one workgroup per pair, 300 sequences of 1 .. 700 keys, 16 heads of 64:
+// 42 us for 198 MB, 4.7 TB/s; three sequences of 40000 .. 120000 keys, 48 / 4 heads of 256: 88 us for 492 MB, 5.6 TB/s.  What
+// carries it:
+//   * Codes are read once and past the caches (load_once), whole 128-byte lines of an instruction: 6.5 TB/s and not 5.9 for
+//     loads alone.  Lines that two instructions halve must stay in the cache between them, so a row narrower than a line is
+//     not split over instructions.
+//   * e4m3 becomes bf16 or fp16 exactly, two numbers per instruction, so the codes are converted in registers in front of the
+//     matrix product, and whatever passes through LDS does so as codes, half the bytes.  One of the two operands passes: the
+//     keys of wide rows (D >= 128), loaded as rows and read as the product wants them; the values of narrow ones.  The other
+//     is loaded as the product wants it, because the order of the contraction index of a product, and of its rows, is free
+//     as long as both operands (and the reader of the result) agree on it.
 //   * The scales never touch the codes: ks multiplies the scores, vs the probabilities.
 //   * S^T = K Q^T (keys x queries) by 16x16x32 products, as in decode.hpp: lane l = 16 g + i.  Row i of score block kb of a
 //     group of 32 keys is key 8 (i / 4) + 4 kb + i % 4, so that lane (g, i) of the result has keys 8g + 4kb + 0..3 of query
@@ -14,10 +21,17 @@
 //     8g + e.  The A operand is eight keys' codes of one value index d: lane (g, i) loads, of each of its eight keys, the
 //     D / 16 codes that start at d = i D / 16, and pairs the codes of two keys by byte selection before converting them.
 //     (At D = 512: 16 codes from 16 i and 16 from 256 + 16 i.)
-//   * The eight keys of a lane lie in one cache block where the block size is a power of two of at least eight: one table
-//     entry, one address and two scales for all of them.  Other block sizes look up every key.
+//   * Eight keys from a multiple of eight on lie in one cache block where the block size is a power of two of at least eight:
+//     one table entry, one address and two scales for all of them, and whole rows that a load instruction of all lanes takes
+//     from one scalar address.  With other block sizes every lane looks up one key of a step, and the lanes that need its
+//     block, row or scale get them by an exchange (the 64 sequences in blocks of 32: 105 us, of 24: 113).
+//   * The chain table -> codes is a step long: entries are requested a step ahead of the codes that they lead to, between the
+//     loads of this step's keys and values, since loads return in order and waiting for a later one waits for all before it.
 //   * The reference of the exponentials is raised only when a score passes it by more than 2^8 (base 2): most steps need
 //     no exchange between lanes.
+//   * Many pairs that are cut: a range of keys to every wavefront, no barrier from the first load to the last store (100 us
+//     for the 64 sequences and their merge, 124 with a range to every workgroup).  Few pairs: pieces to workgroups, which leave a quarter of the
+//     partial results.  Short sequences: a workgroup per pair, one kernel.  (choose_workgroups in paged_fp8.py has the rule.)
 //
 // A table entry outside the cache (or a column behind the table) makes its keys' scores NaN, and with them the rows that
 // see them; nothing is read outside the cache.
@@ -92,8 +106,6 @@ struct E4m3Source {
     const int sign = entry_shift == 3 ? 0 : e.lo;
     return e.inside && e.hi == sign && (uint32_t)e.lo < (uint32_t)num_blocks ? e.lo : -1;
   }
-  // any block size
-  FA_DEVICE int block_of_key(int n) const { return block(request(n / bs)); }
 };
 
 // Un-normalised result of a wavefront: lane (g, i) has values e4m3_value_index(4g + r, u) of query row i in o[u][r],
@@ -117,13 +129,20 @@ FA_DEVICE void decode_e4m3(const E4m3Source& src, const T* q_row /* query row of
   const int tid = hw::thread_id(), lane = tid & 63, patch_index = hw::uniform(tid >> 6), wave = WAVES > 1 ? patch_index : 0;
   const int li = lane & 15, g = lane >> 4;
 
-  // OCTETS: lane o has the table's entry for octet o of a step, requested a step ahead and resolved when its keys are fetched.
+  // OCTETS: lane o has the table's entry for octet o of a step, otherwise lane n that for key n and the key's row in its block;
+  // requested a step ahead and resolved when its keys are fetched.
   // (The first is requested in front of everything else: the context length, which bounds the steps, may still be on its way.
   // Entries behind it are columns like others, and not used.)
   E4m3Source::Entry ahead = {0, 0, 0};
-  int octet_block = 0;
+  int found_block = 0, found_row = 0, ahead_row = 0;
   auto lookup = [&](int n0) {
-    if constexpr (OCTETS) ahead = src.request((n0 + 8 * (lane & (C::TK / 8 - 1))) >> src.bs_shift);
+    if constexpr (OCTETS) {
+      ahead = src.request((n0 + 8 * (lane & (C::TK / 8 - 1))) >> src.bs_shift);
+    } else {
+      const uint32_t n = n0 + (lane & (C::TK - 1)), column = n / (uint32_t)src.bs;
+      ahead = src.request((int)column);
+      ahead_row = (int)(n - column * (uint32_t)src.bs);
+    }
   };
   lookup(n_begin + wave * C::TK);
 
@@ -156,12 +175,20 @@ FA_DEVICE void decode_e4m3(const E4m3Source& src, const T* q_row /* query row of
   auto k_key = [&](int n0, int kb) { return n0 + 8 * (li >> 2) + 4 * kb + (li & 3); };
   auto v_key = [&](int n0, int e) { return n0 + 8 * g + e; };
   uint32_t kw[2][C::KW], vw[8][C::VW], sw[2][C::STAGE_K ? 1 : C::KW];
-  constexpr int NV = OCTETS ? 1 : 8;   // scales that a lane needs
-  float ksc[NV], vsc[NV];
+  float ksc = 0.f, vsc = 0.f;   // scales of the lane's octet, or of its key
+  // Element offset of a row (key of the step, at most the last), where a lane's rows are not those of one octet: the block and
+  // the row in it from the lane that has looked them up.
+  auto row_at = [&](int key) {
+    return (int64_t)imax(hw::lane_value(found_block, key), 0) * src.s_blk + (int64_t)hw::lane_value(found_row, key) * src.s_tok;
+  };
+  auto scale_of = [&](float scale, int key) {
+    return OCTETS ? scale : hw::lane_value(scale, key);
+  };
   unsigned char* patch = smem + patch_index * C::PATCH;
   auto fetch_k = [&](int n0) {
     const uint32_t s_tok = (uint32_t)src.s_tok;
-    if constexpr (OCTETS) octet_block = src.block(ahead);
+    found_block = src.block(ahead);
+    found_row = ahead_row;
     if constexpr (C::STAGE_K) {
       const uint32_t col = 16 * (lane % CPR);
       if (OCTETS && n0 + C::TK <= n_end) {
@@ -169,25 +196,27 @@ FA_DEVICE void decode_e4m3(const E4m3Source& src, const T* q_row /* query row of
 #pragma unroll
         for (int i = 0; i < C::NKI; ++i) {   // the keys of an instruction lie in one octet: one address for all lanes
           const int n = n0 + i * C::RPI;
-          const int64_t at = (int64_t)imax(hw::read_lane(octet_block, i * C::RPI / 8), 0) * src.s_blk + (int64_t)(n & (src.bs - 1)) * src.s_tok;
+          const int64_t at = (int64_t)imax(hw::read_lane(found_block, i * C::RPI / 8), 0) * src.s_blk + (int64_t)(n & (src.bs - 1)) * src.s_tok;
           load_codes<16>(src.kc + at + off, &kw[0][0] + 4 * i);
         }
       } else {
 #pragma unroll
         for (int i = 0; i < C::NKI; ++i) {
-          const int n = imin(n0 + i * C::RPI + lane / CPR, last);
-          const int b = OCTETS ? hw::lane_value(octet_block, (n - n0) >> 3) : src.block_of_key(n);
-          load_codes<16>(src.kc + (int64_t)imax(b, 0) * src.s_blk + (int64_t)(OCTETS ? n & (src.bs - 1) : n % src.bs) * src.s_tok + col,
-                         &kw[0][0] + 4 * i);
+          const int key = imin(i * C::RPI + lane / CPR, last - n0);
+          int64_t at;
+          if constexpr (OCTETS) at = (int64_t)imax(hw::lane_value(found_block, key >> 3), 0) * src.s_blk + (int64_t)((n0 + key) & (src.bs - 1)) * src.s_tok;
+          else at = row_at(key);
+          load_codes<16>(src.kc + at + col, &kw[0][0] + 4 * i);
         }
       }
     } else {
-      const int at_octet = OCTETS ? hw::lane_value(octet_block, imin(li >> 2, (last - n0) >> 3)) : 0;
+      const int64_t octet_at = OCTETS ? (int64_t)imax(hw::lane_value(found_block, imin(li >> 2, (last - n0) >> 3)), 0) * src.s_blk : 0;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        const int n = imin(k_key(n0, kb), last);
-        const int b = OCTETS ? at_octet : src.block_of_key(n);
-        const int64_t at = (int64_t)imax(b, 0) * src.s_blk + (int64_t)(OCTETS ? n & (src.bs - 1) : n % src.bs) * src.s_tok + C::KB_BYTES * g;
+        const int key = imin(k_key(0, kb), last - n0);
+        int64_t at = C::KB_BYTES * g;
+        if constexpr (OCTETS) at += octet_at + (int64_t)((n0 + key) & (src.bs - 1)) * src.s_tok;
+        else at += row_at(key);
         load_codes<C::KB_BYTES>(src.kc + at, kw[kb]);
         load_codes<C::KB_BYTES>(src.vc + at, sw[kb]);
       }
@@ -196,29 +225,25 @@ FA_DEVICE void decode_e4m3(const E4m3Source& src, const T* q_row /* query row of
   // (behind fetch_k of the same step)
   auto fetch_v = [&](int n0) {
     const bool full = n0 + C::TK <= n_end;
-    int blk[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int b = OCTETS ? hw::lane_value(octet_block, imin(g, (last - n0) >> 3)) : src.block_of_key(imin(v_key(n0, i), last));
-      blk[i] = imax(b, 0);
-      const float k = src.ks[(int64_t)blk[i] * src.s_scale], v = src.vs[(int64_t)blk[i] * src.s_scale];
-      ksc[i] = b >= 0 ? k : __builtin_nanf("");
-      vsc[i] = v;
-    }
+    const int b = OCTETS ? hw::lane_value(found_block, imin(g, (last - n0) >> 3)) : found_block, blk = imax(b, 0);
+    const float k = src.ks[(int64_t)blk * src.s_scale];
+    vsc = src.vs[(int64_t)blk * src.s_scale];
+    ksc = b >= 0 ? k : __builtin_nanf("");
     if constexpr (C::STAGE_K) {
       auto load = [&](int e, const uint8_t* row) {
         load_codes<C::VB_BYTES>(row + (D == 512 ? 16 : C::VB_BYTES) * li, vw[e]);
         if constexpr (D == 512) load_codes<16>(row + 256 + 16 * li, &vw[e][4]);
       };
       if (OCTETS && full) {
-        const uint8_t* row = src.vc + (int64_t)blk[0] * src.s_blk + (int64_t)(v_key(n0, 0) & (src.bs - 1)) * src.s_tok;
+        const uint8_t* row = src.vc + (int64_t)blk * src.s_blk + (int64_t)(v_key(n0, 0) & (src.bs - 1)) * src.s_tok;
 #pragma unroll
         for (int e = 0; e < 8; ++e) load(e, row + e * src.s_tok);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int n = imin(v_key(n0, e), last);
-          load(e, src.vc + (int64_t)blk[OCTETS ? 0 : e] * src.s_blk + (int64_t)(OCTETS ? n & (src.bs - 1) : n % src.bs) * src.s_tok);
+          const int key = imin(v_key(0, e), last - n0);
+          if constexpr (OCTETS) load(e, src.vc + (int64_t)blk * src.s_blk + (int64_t)((n0 + key) & (src.bs - 1)) * src.s_tok);
+          else load(e, src.vc + row_at(key));
         }
       }
     }
@@ -280,7 +305,7 @@ FA_DEVICE void decode_e4m3(const E4m3Source& src, const T* q_row /* query row of
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float t = s[kb][r] * (ksc[OCTETS ? 0 : 4 * kb + r] * c2);
+        float t = s[kb][r] * (scale_of(ksc, imin(v_key(0, 4 * kb + r), last - n0)) * c2);
         t = v_key(n0, 4 * kb + r) < n_end ? t : neg_inf();
         s[kb][r] = t;
         mx = fmaxf(mx, t);
@@ -303,7 +328,7 @@ FA_DEVICE void decode_e4m3(const E4m3Source& src, const T* q_row /* query row of
       for (int r = 0; r < 4; ++r) {
         const float e = hw::exp2_fast(s[kb][r] - m_use);
         l_i += e;
-        const float pv = e * vsc[OCTETS ? 0 : 4 * kb + r];
+        const float pv = e * scale_of(vsc, imin(v_key(0, 4 * kb + r), last - n0));
         p1[4 * kb + r] = (hw::bf16_t)pv;
         if (TWO) p2[4 * kb + r] = (hw::bf16_t)(pv - (float)p1[4 * kb + r]);
       }

@@ -335,6 +335,15 @@ inline int wave_prefix_sum(int x) {
   }
   return x;
 }
+inline float lane_value(float x, int lane) {
+  float result = x;
+  const int me = hwsim::cur & 63;
+  for (int m = 1; m < 64; ++m) {
+    const float got = shfl_xor(x, m);
+    if ((me ^ m) == lane) result = got;
+  }
+  return result;
+}
 inline int lane_value(int x, int lane) {
   int result = x;
   const int me = hwsim::cur & 63;
