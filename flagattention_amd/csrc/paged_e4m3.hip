@@ -30,8 +30,9 @@
 //   * The reference of the exponentials is raised only when a score passes it by more than 2^8 (base 2): most steps need
 //     no exchange between lanes.
 //   * Many pairs that are cut: a range of keys to every wavefront, no barrier from the first load to the last store (100 us
-//     for the 64 sequences and their merge, 124 with a range to every workgroup).  Few pairs: pieces to workgroups, which leave a quarter of the
-//     partial results.  Short sequences: a workgroup per pair, one kernel.  (choose_workgroups in paged_fp8.py has the rule.)
+//     for 64 sequences and their merge, 124 with a range to every workgroup).  Few pairs: pieces to workgroups, which leave a
+//     quarter of the partial results.  Short sequences: a workgroup per pair, one kernel.  (The rule: choose_workgroups in
+//     paged_fp8.py.)
 //
 // A table entry outside the cache (or a column behind the table) makes its keys' scores NaN, and with them the rows that
 // see them; nothing is read outside the cache.

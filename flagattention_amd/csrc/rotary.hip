@@ -11,7 +11,10 @@
 // reads dy alone); the tables are read once per token and group of heads, from the caches.  So nothing is staged: a row is
 // held by D / 16 lanes, each with eight values of the first half of the turned part and the eight they are paired with (the
 // rest of the row is dealt the same way), which makes both kinds of pairs local to a lane and the mean a few lane exchanges.
-// A wavefront holds 1024 / D tokens at a time and walks a run of heads with their cosines and sines in registers.
+// A wavefront holds 1024 / D tokens at a time and walks a run of heads with their cosines and sines in registers, the next
+// head's row on its way.  8192 tokens, 32 + 8 heads of 128, bf16: forward 31 us (172 MB, 5.5 TB/s; a copy of that size
+// reaches 4.8 to 6.9, as much of it as the last-level cache holds), backward with weights 50 + 4 us (252 MB); 64 single
+// tokens 4.7 us, latency.
 #include "rotary.hpp"
 
 namespace fa {
