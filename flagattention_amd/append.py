@@ -26,6 +26,12 @@ def tables_ready(cos, sin, head_size, device):
     return cos, sin
 
 
+def check_written(a, b, name):
+    """A pair of tensors that a call writes to."""
+    assert a.data_ptr() != b.data_ptr() or a.numel() == 0, f"key_{name} and value_{name} must be tensors of their own"
+    assert not any(s == 0 and n > 1 for s, n in zip(a.stride(), a.shape)), f"{name} to be written to must not be expanded"
+
+
 def append(key, value, key_cache, value_cache, context_lens, block_tables, query_starts=None, key_scales=None,
            value_scales=None, cos=None, sin=None, interleaved=False):
     """Stores ``key`` and ``value`` (rows, heads_kv, head_size), float16 or bfloat16, in ``key_cache`` and ``value_cache``
@@ -58,10 +64,12 @@ def append(key, value, key_cache, value_cache, context_lens, block_tables, query
     assert key_cache.shape[1] == num_kv_heads and key_cache.shape[3] == head_size, \
         f"rows of {num_kv_heads} heads of {head_size}, and a cache of {tuple(key_cache.shape)}"
     assert head_size in _HEAD_SIZES, f"head_size={head_size}"
+    check_written(key_cache, value_cache, "cache")
     assert (key_scales is None) == (value_scales is None), "key_scales and value_scales: both or neither"
     tensors = [value, key_cache, value_cache, block_tables]
     if key_scales is not None:
         check_cache(key_cache, value_cache, key_scales, value_scales)
+        check_written(key_scales, value_scales, "scales")
         tensors += [key_scales, value_scales]
     else:
         assert key_cache.dtype == value_cache.dtype == key.dtype, \

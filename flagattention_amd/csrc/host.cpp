@@ -833,6 +833,14 @@ PyObject* paged_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// append.check_written
+bool written_ok(const Tensor& a, const Tensor& b) {
+  if (a.const_data_ptr() == b.const_data_ptr()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) == 0) return false;
+  return true;
+}
+
 // paged_append(key, value, key_cache, value_cache, context_lens, block_tables, query_starts, key_scales, value_scales, cos, sin,
 //              interleaved)
 PyObject* paged_append_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -848,13 +856,13 @@ PyObject* paged_append_call(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int interleaved = PyObject_IsTrue(a[11]);
   if (interleaved < 0) throw python_error();
   if (!k.is_cuda() || v.device() != k.device() || !rows3_ready(k) || !rows3_ready(v) || !type_ok(k) || v.scalar_type() != k.scalar_type() ||
-      v.sizes() != k.sizes() || !caches_ok(kc, vc, k))
+      v.sizes() != k.sizes() || !caches_ok(kc, vc, k) || !written_ok(kc, vc))
     return not_taken();
   const int64_t rows = k.size(0), Hkv = k.size(1), D = k.size(2), seqs = bt.dim() == 2 ? bt.size(0) : 0;
   if (!fits_int({rows, Hkv, seqs}) || kc.size(1) != Hkv || kc.size(3) != D || !head_size_ok(D) || !table_ready(bt, k, seqs) ||
       !int32_ready(lens, k, seqs) || (starts ? !int32_ready(*starts, k, seqs + 1) : rows != seqs))
     return not_taken();
-  if ((ks == nullptr) != (vs == nullptr) || (ks ? !scales_ok(kc, *ks, *vs) : kc.scalar_type() != k.scalar_type())) return not_taken();
+  if ((ks == nullptr) != (vs == nullptr) || (ks ? !scales_ok(kc, *ks, *vs) || !written_ok(*ks, *vs) : kc.scalar_type() != k.scalar_type())) return not_taken();
   if ((cos == nullptr) != (sin == nullptr) || (cos && !tables_ready(*cos, *sin, k, D))) return not_taken();
   {
     pybind11::gil_scoped_release no_gil;

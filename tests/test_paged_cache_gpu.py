@@ -51,6 +51,15 @@ def test_lengths_far_past_the_table_end_soon():
         assert out[0].isnan().all() and out[2].isnan().all() and out[1].isfinite().all(), longest
 
 
+def test_append_refuses_what_it_would_write_to_twice():
+    good = cases.append_inputs(FP16, 8, [3, 9], [4, 7], 2, 64, 16, 64, 26, device="cuda")
+    ones = [torch.ones(1, 1, device="cuda").expand(*good["key_scales"].shape) for _ in range(2)]
+    for change in (dict(value_cache=good["key_cache"]), dict(value_scales=good["key_scales"]), dict(key_scales=ones[0], value_scales=ones[1])):
+        with pytest.raises(AssertionError):
+            flag_attn.paged_append(**{**good, **change})
+            pytest.fail(str(list(change)))
+
+
 def test_norm_rotary_is_differentiable_once():
     args = cases.rotary_inputs(BF16, 1, 2, 2, 6, 64, 64, 37, device="cuda", grad=True)
     q, k = flag_attn.norm_rotary(**args)

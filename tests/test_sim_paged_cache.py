@@ -249,6 +249,17 @@ def test_append_refuses():
         assert torch.equal(before.view(torch.uint8), a["key_cache"].view(torch.uint8))
 
 
+def test_append_refuses_what_it_would_write_to_twice():
+    good = cases.append_inputs(FP16, 8, [3, 9], [4, 7], 2, 64, 16, 64, 26)
+    one = torch.ones(1, 1).expand(*good["key_scales"].shape)
+    for change in (dict(value_cache=good["key_cache"]), dict(value_scales=good["key_scales"]),
+                   dict(key_scales=one, value_scales=one.clone().expand_as(one)), dict(key_scales=one, value_scales=one * 1),
+                   {n: torch.zeros_like(good["key_cache"])[:1].expand_as(good["key_cache"]) for n in ("key_cache", "value_cache")}):
+        with pytest.raises(AssertionError):
+            flag_attn.paged_append(**{**good, **change})
+            pytest.fail(str(list(change)))
+
+
 def test_append_of_nothing():
     args = cases.append_inputs(FP16, 8, [3, 9], [4, 7], 2, 64, 16, 64, 27)
     for change in (dict(key=args["key"][:0], value=args["value"][:0], query_starts=torch.zeros(3, dtype=torch.int32)),
