@@ -71,10 +71,14 @@ FA_KERNEL void FA_LAUNCH_BOUNDS(kThreads) append_kernel(AppendParams p) {
   const int h0 = item % chunks * p.heads_per_item, h1 = imin(h0 + p.heads_per_item, p.Hkv);
   const int64_t row0 = (int64_t)(item / chunks) * (1024 / D), row = row0 + lane / (D / 16);
   int s = (int)row;
-  if (p.starts) {   // the first row's sequence, and from there to the lane's own
+  if (p.starts) {   // the first row's sequence, and from there to the lane's own in growing and then in shrinking steps
     s = last_not_above(p.num_seqs, row0, lane, [&](int i) { return (int64_t)p.starts[i]; });
     if (s < 0) s = 0;
-    while (s + 1 < p.num_seqs && p.starts[s + 1] <= row) ++s;
+    int step = 1;
+    auto reaches = [&]() { return step < p.num_seqs - s && p.starts[s + step] <= row; };
+    for (; reaches(); step *= 2) s += step;
+    for (step /= 2; step > 0; step /= 2)
+      if (reaches()) s += step;
   }
   if (row >= p.rows || s >= p.num_seqs) return;
   const NewRows rows = new_rows(p, s);

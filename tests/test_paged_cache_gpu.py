@@ -114,6 +114,12 @@ def test_append_to_many_sequences(bits):
     cases.check_append(cases.append_inputs(BF16, bits, olds, news, 2, 64, 16, 64, 22, device="cuda", pad=9))
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+def test_append_past_many_empty_sequences(bits):
+    news = [3, 1, 1] + [0] * 700 + [2] + [0] * 50 + [1, 0, 9] + [0] * 300
+    cases.check_append(cases.append_inputs(FP16, bits, [(3 * i) % 7 for i in range(len(news))], news, 2, 64, 8, 32, 29, device="cuda", pad=4))
+
+
 @pytest.mark.parametrize("rotary", [0, 32, 48, 128])
 @pytest.mark.parametrize("olds,news,block", [
     ([(7 * i) % 40 for i in range(80)], [(11 * i) % 60 for i in range(80)], 16),     # a wavefront for a block of a head

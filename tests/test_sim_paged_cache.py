@@ -172,6 +172,12 @@ def test_append_by_wavefronts():
     cases.check_append(args)
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+def test_append_past_many_empty_sequences(bits):
+    news = [3, 1, 1] + [0] * 37 + [2] + [0] * 5 + [1, 0, 9, 0, 0]
+    cases.check_append(cases.append_inputs(FP16, bits, [(3 * i) % 7 for i in range(len(news))], news, 1, 64, 8, 32, 29, pad=4))
+
+
 def test_append_makes_room_for_larger_values():
     """Values far above what the block holds: the scale grows, what is there is rounded again, to zero where it falls short."""
     for values in (1e-3, 40.0, 3e4):
